@@ -146,6 +146,81 @@ int tsn_rope_pairs(tsn_runtime *rt, float *x, const int32_t *pos, uint32_t rows,
 int tsn_attention(tsn_runtime *rt, const float *qkv, float *out, uint32_t S, uint32_t nh, uint32_t hd, uint32_t ld,
                   uint32_t ldo, uint32_t q_off, uint32_t k_off, uint32_t v_off, uint32_t o_off, float scale);
 
+/* ---------------- transformer block operators beside the launchers above (no reference counterpart) ----------------
+ * Inference forms, all on the runtime's stream, none allocating device memory. Each reads its spec (host memory)
+ * before it returns. Argument errors are found before anything is launched. */
+
+/* Rotary positions with several axes (time, height, width): tsn_rope_pairs for clip rows cut from frames. Pair i of
+ * axis a of every head of row r turns by
+ *     pos[r % pos_rows][a] * fscale[a] * base[a]^(-2i / dim[a]),
+ * the angle in 64 bits, reduced before its sine and cosine are taken in 32. The axes' elements follow each other
+ * in a head: axis a's segment starts at dim[0] + .. + dim[a-1]; what is behind the last is copied. y may be x (same
+ * row stride); otherwise their elements must not overlap. n_axes = 1, dim = hd is tsn_rope_pairs. */
+typedef struct {
+    int dtype;                    /* elements of x and y: TSN_F32, TSN_F16 or TSN_BF16 */
+    uint32_t rows, nh, hd;        /* rows of nh heads of hd elements (even, at most 256) */
+    uint32_t ldx, ldy;            /* row strides in elements; 0: nh*hd */
+    uint32_t pos_rows;            /* rows of pos, shared by the samples of a batch; 0: rows */
+    uint32_t n_axes;              /* 1 to 4 */
+    uint32_t dim[4];              /* elements of a head that each axis turns (even, 0 allowed; together at most hd) */
+    float base[4], fscale[4];     /* base > 0 */
+    int half_split;               /* 0: pairs (2i, 2i+1) of a segment; 1: pairs (i, i + dim/2) */
+    int inverse;                  /* 1: turns back */
+} tsn_rope_axes_spec;
+/* pos [pos_rows][n_axes] */
+int tsn_rope_axes(tsn_runtime *rt, const tsn_rope_axes_spec *spec, const void *x, const int32_t *pos, void *y);
+
+/* Differential attention: the difference of two softmax maps, per head h with its key/value head g = h*nkv/nh,
+ *     lambda = exp(lq1.lk1) - exp(lq2.lk2) + lambda_init        lam = [lam_heads][lq1, lk1, lq2, lk2][hd]
+ *     o = (softmax(scale q1 k1^T) - lambda softmax(scale q2 k2^T)) v
+ *     out = norm_w ? (1 - lambda_init) * o / sqrt(mean(o^2) + eps) * norm_w : o
+ * q row: head h's two maps at columns 2h*hd and (2h+1)*hd; k row: g's at 2g*hd and (2g+1)*hd; v and out rows: 2*hd
+ * columns a head. hd is 32 or 64; lambda_init in [0, 1).
+ * q_len, kv_len (device, [B], null: Sq, Sk; values are taken as 0 to Sq, 0 to Sk): row i < q_len of a sample sees
+ * keys j < kv_len, with causal only j <= i + kv_len - q_len (its rows are the last of its keys, as new rows behind
+ * a cache are). A row that sees no key gives zeros. Rows of out from q_len on are left as they were. k and v rows
+ * from kv_len on may hold anything, infinities and NaN among it; those before are finite.
+ * f16 or bf16 in and out; scores, softmax statistics and sums in f32, probabilities rounded to the inputs' type for
+ * the product with v. 16-byte aligned pointers and strides of a multiple of 8 elements run on MFMA, others a plain
+ * kernel. out must not overlap an input. Partial results of long keys over few rows go to the runtime's 32 MiB
+ * workspace and are joined in a fixed order: same bits on every run. */
+typedef struct {
+    int dtype;                    /* q, k, v and out: TSN_F16 or TSN_BF16 */
+    uint32_t B, Sq, Sk;           /* samples, rows and keys of each */
+    uint32_t nh, nkv, hd;         /* differential heads, key/value heads (nh a multiple), width of one map */
+    uint32_t ldq, ldk, ldv, ldo;  /* row strides in elements; 0: packed (2*nh*hd or 2*nkv*hd) */
+    uint64_t bsq, bsk, bsv, bso;  /* sample strides in elements; 0: S * ld */
+    uint32_t lam_heads;           /* lambda vectors: 1 (shared) or nh */
+    int causal;
+    float scale, lambda_init, eps;
+} tsn_diff_attn_spec;
+int tsn_diff_attention(tsn_runtime *rt, const tsn_diff_attn_spec *spec, const void *q, const void *k, const void *v,
+                       const float *lam, const float *norm_w, const int32_t *q_len, const int32_t *kv_len, void *out);
+
+/* Norms after and before a block fused with its gate and residual scale: gate_add and adaln_ln with weights, in one
+ * pass over the rows:
+ *     z     = post norm of f * post_w + post_b
+ *     x_out = x_scale * x + f_scale * gate * z
+ *     y     = (pre norm of x_out * pre_w + pre_b) * (1 + scale) + shift
+ * The norms are over the H elements of a row (LN: biased variance), in f32; y is made from x_out before its
+ * rounding. gate, shift and scale are chunks (H floats) of row r / mod_rows of mod [][chunks*H]; a chunk of -1 is
+ * absent (gate 1, shift 0, scale 0), mod null if all three are. Weights and biases may be null. y null: x_out only.
+ * x_out may be x and y may be f (same element type and row stride); otherwise outputs overlap nothing. */
+typedef enum { TSN_NORM_NONE = 0, TSN_NORM_RMS = 1, TSN_NORM_LN = 2 } tsn_norm;
+typedef struct {
+    uint32_t rows, H;             /* H at most 16384 */
+    int x_dtype, f_dtype, y_dtype; /* x and x_out; f; y: TSN_F32, TSN_F16 or TSN_BF16 */
+    int post, pre;                /* tsn_norm */
+    uint32_t ldx, ldf, ldo, ldy;  /* row strides in elements; 0: H */
+    float x_scale, f_scale;
+    uint32_t chunks, mod_rows;    /* mod_rows: consecutive rows that share a row of mod; 0: all */
+    int gate, shift, scale;       /* chunk indices or -1 */
+    float post_eps, pre_eps;
+} tsn_gate_norm_spec;
+int tsn_gate_add_norm(tsn_runtime *rt, const tsn_gate_norm_spec *spec, const void *x, const void *f, const float *mod,
+                      const float *post_w, const float *post_b, const float *pre_w, const float *pre_b, void *x_out,
+                      void *y);
+
 /* Calibration (no reference counterpart: it measures the denominators a roofline is quoted
  * against). Sustained dense f16 MFMA rate (about 20 ms of one workgroup of 8 waves per CU running
  * independent v_mfma_f32_16x16x32_f16 chains), and device copy bandwidth (read + write of 1 GiB), both timed with

@@ -17,6 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libtsn.so")
 
 F32, F16, BF16 = 0, 1, 2
+NORM_NONE, NORM_RMS, NORM_LN = 0, 1, 2
 _NP_DT = {F32: np.float32, F16: np.float16, BF16: np.uint16}
 
 _lib = None
@@ -133,6 +134,34 @@ class RefCondSpec(ctypes.Structure):
         return s
 
 
+class RopeAxesSpec(ctypes.Structure):
+    """tsn_rope_axes_spec (include/tsn.h)."""
+    _fields_ = [("dtype", ctypes.c_int), ("rows", ctypes.c_uint32), ("nh", ctypes.c_uint32), ("hd", ctypes.c_uint32),
+                ("ldx", ctypes.c_uint32), ("ldy", ctypes.c_uint32), ("pos_rows", ctypes.c_uint32),
+                ("n_axes", ctypes.c_uint32), ("dim", ctypes.c_uint32 * 4), ("base", ctypes.c_float * 4),
+                ("fscale", ctypes.c_float * 4), ("half_split", ctypes.c_int), ("inverse", ctypes.c_int)]
+
+
+class DiffAttnSpec(ctypes.Structure):
+    """tsn_diff_attn_spec (include/tsn.h)."""
+    _fields_ = [("dtype", ctypes.c_int), ("B", ctypes.c_uint32), ("Sq", ctypes.c_uint32), ("Sk", ctypes.c_uint32),
+                ("nh", ctypes.c_uint32), ("nkv", ctypes.c_uint32), ("hd", ctypes.c_uint32),
+                ("ldq", ctypes.c_uint32), ("ldk", ctypes.c_uint32), ("ldv", ctypes.c_uint32), ("ldo", ctypes.c_uint32),
+                ("bsq", ctypes.c_uint64), ("bsk", ctypes.c_uint64), ("bsv", ctypes.c_uint64), ("bso", ctypes.c_uint64),
+                ("lam_heads", ctypes.c_uint32), ("causal", ctypes.c_int), ("scale", ctypes.c_float),
+                ("lambda_init", ctypes.c_float), ("eps", ctypes.c_float)]
+
+
+class GateNormSpec(ctypes.Structure):
+    """tsn_gate_norm_spec (include/tsn.h)."""
+    _fields_ = [("rows", ctypes.c_uint32), ("H", ctypes.c_uint32), ("x_dtype", ctypes.c_int), ("f_dtype", ctypes.c_int),
+                ("y_dtype", ctypes.c_int), ("post", ctypes.c_int), ("pre", ctypes.c_int), ("ldx", ctypes.c_uint32),
+                ("ldf", ctypes.c_uint32), ("ldo", ctypes.c_uint32), ("ldy", ctypes.c_uint32),
+                ("x_scale", ctypes.c_float), ("f_scale", ctypes.c_float), ("chunks", ctypes.c_uint32),
+                ("mod_rows", ctypes.c_uint32), ("gate", ctypes.c_int), ("shift", ctypes.c_int), ("scale", ctypes.c_int),
+                ("post_eps", ctypes.c_float), ("pre_eps", ctypes.c_float)]
+
+
 class KernelStat(ctypes.Structure):
     """tsn_kernel_stat (include/tsn.h)."""
     _fields_ = [("name", ctypes.c_char * 64), ("launches", ctypes.c_int), ("total_ms", ctypes.c_double),
@@ -180,6 +209,9 @@ _SIGS = {
     "tsn_rms_head": [_P, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _FL],
     "tsn_rope_pairs": [_P, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _FL, _FL],
     "tsn_attention": [_P, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _U32, _U32, _U32, _FL],
+    "tsn_rope_axes": [_P, ctypes.POINTER(RopeAxesSpec), _P, _P, _P],
+    "tsn_diff_attention": [_P, ctypes.POINTER(DiffAttnSpec), _P, _P, _P, _P, _P, _P, _P, _P],
+    "tsn_gate_add_norm": [_P, ctypes.POINTER(GateNormSpec), _P, _P, _P, _P, _P, _P, _P, _P, _P],
     "tsn_dit_default_spec": [_I, ctypes.POINTER(DitSpec)],
     "tsn_dit_manifest_count": [ctypes.POINTER(DitSpec)],
     "tsn_dit_manifest_entry": [ctypes.POINTER(DitSpec), _I, ctypes.c_char_p, _I,
@@ -341,6 +373,33 @@ def default_spec(workload):
     s = DitSpec()
     call("tsn_dit_default_spec", workload, ctypes.byref(s))
     return s
+
+
+def rope_axes_spec(dtype, rows, nh, hd, dims, bases, fscales=None, ldx=0, ldy=0, pos_rows=0, half_split=False,
+                   inverse=False):
+    """Rotary positions over len(dims) axes: axis a turns dims[a] elements of a head, at fscales[a] (1) times
+    bases[a]^(-2i/dims[a]) a position."""
+    n = len(dims)
+    if not 1 <= n <= 4 or len(bases) != n or (fscales is not None and len(fscales) != n):
+        raise ValueError("rope_axes: one to four axes, a base (and scale) for each")
+    a4 = lambda t, v: (t * 4)(*v, *([0] * (4 - n)))  # noqa: E731
+    return RopeAxesSpec(dtype, rows, nh, hd, ldx, ldy, pos_rows, n, a4(ctypes.c_uint32, dims), a4(ctypes.c_float, bases),
+                        a4(ctypes.c_float, fscales or [1.0] * n), int(half_split), int(inverse))
+
+
+def diff_attn_spec(dtype, B, Sq, Sk, nh, nkv, hd, causal=False, scale=None, lambda_init=0.8, eps=1e-5, lam_heads=1,
+                   ldq=0, ldk=0, ldv=0, ldo=0, bsq=0, bsk=0, bsv=0, bso=0):
+    """Differential attention of nh heads (two maps of width hd, values of 2*hd) over nkv key/value heads."""
+    return DiffAttnSpec(dtype, B, Sq, Sk, nh, nkv, hd, ldq, ldk, ldv, ldo, bsq, bsk, bsv, bso, lam_heads, int(causal),
+                        hd ** -0.5 if scale is None else scale, lambda_init, eps)
+
+
+def gate_norm_spec(rows, H, x_dtype=F32, f_dtype=F32, y_dtype=F32, post=NORM_RMS, pre=NORM_RMS, x_scale=1.0, f_scale=1.0,
+                   chunks=0, mod_rows=0, gate=-1, shift=-1, scale=-1, post_eps=1e-5, pre_eps=1e-5, ldx=0, ldf=0, ldo=0,
+                   ldy=0):
+    """Norms after and before a block with its gate and residual scale; chunk indices of -1 are absent."""
+    return GateNormSpec(rows, H, x_dtype, f_dtype, y_dtype, post, pre, ldx, ldf, ldo, ldy, x_scale, f_scale, chunks,
+                        mod_rows, gate, shift, scale, post_eps, pre_eps)
 
 
 def manifest(spec):
@@ -932,6 +991,44 @@ class Runtime:
     def attention(self, qkv, out, S, nh, hd, ld, ldo, q_off, k_off, v_off, o_off, scale):
         call("tsn_attention", self.h, qkv.p, out.p, S, nh, hd, ld, ldo, q_off, k_off, v_off, o_off, scale)
 
+    # --- block operators: device arrays, and a spec made once (rope_axes_spec, diff_attn_spec, gate_norm_spec) ---
+    def rope_axes(self, spec, x, pos, y):
+        """multi-axis rotary positions of the heads in x's rows, to y (which may be x)"""
+        n = spec.rows and spec.nh * spec.hd
+        size = 4 if spec.dtype == F32 else 2
+        _need("rope_axes: x", x, _span(spec.rows, spec.ldx or n, n), size)
+        _need("rope_axes: pos", pos, (spec.pos_rows or spec.rows) * spec.n_axes)
+        _need("rope_axes: y", y, _span(spec.rows, spec.ldy or n, n), size)
+        call("tsn_rope_axes", self.h, spec, x.p, pos.p, y.p)
+
+    def diff_attention(self, spec, q, k, v, lam, norm_w, q_len, kv_len, out):
+        """differential attention; norm_w, q_len and kv_len may be None"""
+        s = spec
+        wq, wk = 2 * s.nh * s.hd, 2 * s.nkv * s.hd
+        _need("diff_attention: q", q, _span3(s.B, s.Sq, s.ldq or wq, s.bsq, wq), 2)
+        _need("diff_attention: k", k, _span3(s.B, s.Sk, s.ldk or wk, s.bsk, wk), 2)
+        _need("diff_attention: v", v, _span3(s.B, s.Sk, s.ldv or wk, s.bsv, wk), 2)
+        _need("diff_attention: out", out, _span3(s.B, s.Sq, s.ldo or wq, s.bso, wq), 2)
+        _need("diff_attention: lam", lam, 4 * s.lam_heads * s.hd)
+        _need("diff_attention: norm_w", norm_w, 2 * s.hd, optional=True)
+        _need("diff_attention: q_len", q_len, s.B, optional=True)
+        _need("diff_attention: kv_len", kv_len, s.B, optional=True)
+        call("tsn_diff_attention", self.h, s, q.p, k.p, v.p, lam.p, _p(norm_w), _p(q_len), _p(kv_len), out.p)
+
+    def gate_add_norm(self, spec, x, f, mod, x_out, y, post_w=None, post_b=None, pre_w=None, pre_b=None):
+        """x_out = x_scale*x + f_scale*gate*post(f), y = pre(x_out)*(1 + scale) + shift; y and mod may be None"""
+        s = spec
+        size = lambda dt: 4 if dt == F32 else 2  # noqa: E731
+        _need("gate_add_norm: x", x, _span(s.rows, s.ldx or s.H, s.H), size(s.x_dtype))
+        _need("gate_add_norm: f", f, _span(s.rows, s.ldf or s.H, s.H), size(s.f_dtype))
+        _need("gate_add_norm: x_out", x_out, _span(s.rows, s.ldo or s.H, s.H), size(s.x_dtype))
+        _need("gate_add_norm: y", y, _span(s.rows, s.ldy or s.H, s.H), size(s.y_dtype), optional=True)
+        _need("gate_add_norm: mod", mod, (-(-s.rows // s.mod_rows) if s.mod_rows else 1) * s.chunks * s.H, optional=True)
+        for name, w in (("post_w", post_w), ("post_b", post_b), ("pre_w", pre_w), ("pre_b", pre_b)):
+            _need("gate_add_norm: " + name, w, s.H, optional=True)
+        call("tsn_gate_add_norm", self.h, s, x.p, f.p, _p(mod), _p(post_w), _p(post_b), _p(pre_w), _p(pre_b), x_out.p,
+             _p(y))
+
     def silu(self, x, n):
         call("tsn_silu", self.h, x.p, n)
 
@@ -969,6 +1066,19 @@ def _need(what, arr, numel, itemsize=4, optional=False):
         raise TypeError("%s: expected a DeviceArray, got %r" % (what, type(arr)))
     if have < numel * itemsize:
         raise ValueError("%s: %d bytes needed, the array holds %d" % (what, numel * itemsize, have))
+
+
+def _p(arr):
+    return None if arr is None else arr.p
+
+
+def _span(rows, ld, width):
+    """elements from the first to the last of rows of width, ld apart"""
+    return (rows - 1) * ld + width if rows else 0
+
+
+def _span3(B, S, ld, bs, width):
+    return (B - 1) * (bs or S * ld) + _span(S, ld, width) if B and S else 0
 
 
 class DitModel:

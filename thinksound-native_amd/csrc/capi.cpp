@@ -256,6 +256,49 @@ int tsn_attention(tsn_runtime *rt, const float *qkv, float *out, uint32_t S, uin
     return rt->rt.attention(qkv, out, S, nh, hd, ld, ldo, q_off, k_off, v_off, o_off, scale);
 }
 
+// The block operators check their arguments before the handle, so every refusal can be seen without a device.
+int tsn_rope_axes(tsn_runtime *rt, const tsn_rope_axes_spec *c, const void *x, const int32_t *pos, void *y) {
+    if (!c) { tsn::set_error("rope_axes: null spec"); return TSN_ERR_ARG; }
+    tsn::RopeAxesArgs a{};
+    a.dt = c->dtype; a.rows = c->rows; a.nh = c->nh; a.hd = c->hd; a.ldx = c->ldx; a.ldy = c->ldy;
+    a.pos_rows = c->pos_rows; a.n_axes = c->n_axes;
+    for (int i = 0; i < 4; ++i) { a.dim[i] = c->dim[i]; a.base[i] = c->base[i]; a.fscale[i] = c->fscale[i]; }
+    a.half_split = c->half_split != 0; a.inverse = c->inverse != 0;
+    a.x = x; a.pos = pos; a.y = y;
+    TSN_TRY(tsn::rope_axes_check(a));
+    RT_CHECK(rt);
+    return rt->rt.rope_axes(a);
+}
+int tsn_diff_attention(tsn_runtime *rt, const tsn_diff_attn_spec *c, const void *q, const void *k, const void *v,
+                       const float *lam, const float *norm_w, const int32_t *q_len, const int32_t *kv_len, void *out) {
+    if (!c) { tsn::set_error("diff_attention: null spec"); return TSN_ERR_ARG; }
+    tsn::DiffAttnArgs a{};
+    a.dt = c->dtype; a.B = c->B; a.Sq = c->Sq; a.Sk = c->Sk; a.nh = c->nh; a.nkv = c->nkv; a.hd = c->hd;
+    a.ldq = c->ldq; a.ldk = c->ldk; a.ldv = c->ldv; a.ldo = c->ldo;
+    a.bsq = c->bsq; a.bsk = c->bsk; a.bsv = c->bsv; a.bso = c->bso;
+    a.lam_heads = c->lam_heads; a.causal = c->causal != 0;
+    a.scale = c->scale; a.lambda_init = c->lambda_init; a.eps = c->eps;
+    a.q = q; a.k = k; a.v = v; a.lam = lam; a.norm_w = norm_w; a.q_len = q_len; a.kv_len = kv_len; a.out = out;
+    TSN_TRY(tsn::diff_attention_check(a));
+    RT_CHECK(rt);
+    return rt->rt.diff_attention(a);
+}
+int tsn_gate_add_norm(tsn_runtime *rt, const tsn_gate_norm_spec *c, const void *x, const void *f, const float *mod,
+                      const float *post_w, const float *post_b, const float *pre_w, const float *pre_b, void *x_out,
+                      void *y) {
+    if (!c) { tsn::set_error("gate_add_norm: null spec"); return TSN_ERR_ARG; }
+    tsn::GateNormArgs a{};
+    a.rows = c->rows; a.H = c->H; a.xdt = c->x_dtype; a.fdt = c->f_dtype; a.ydt = c->y_dtype;
+    a.post = c->post; a.pre = c->pre; a.ldx = c->ldx; a.ldf = c->ldf; a.ldo = c->ldo; a.ldy = c->ldy;
+    a.x_scale = c->x_scale; a.f_scale = c->f_scale; a.chunks = c->chunks; a.mod_rows = c->mod_rows;
+    a.gate = c->gate; a.shift = c->shift; a.scale = c->scale; a.post_eps = c->post_eps; a.pre_eps = c->pre_eps;
+    a.x = x; a.f = f; a.mod = mod; a.post_w = post_w; a.post_b = post_b; a.pre_w = pre_w; a.pre_b = pre_b;
+    a.x_out = x_out; a.y = y;
+    TSN_TRY(tsn::gate_add_norm_check(a));
+    RT_CHECK(rt);
+    return rt->rt.gate_add_norm(a);
+}
+
 int tsn_probe_peaks(tsn_runtime *rt, double *mfma_tflops, double *hbm_gbs) {
     RT_CHECK(rt);
     return rt->rt.probe_peaks(mfma_tflops, hbm_gbs);

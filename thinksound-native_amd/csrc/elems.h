@@ -1,0 +1,45 @@
+// elems.h — element types of the block operators: f32, f16 and bf16 rows as floats, and host checks
+// that two strided row windows share no element.
+#pragma once
+#include "tsn_common.h"
+
+namespace tsn {
+
+typedef __bf16 bf16_t;
+
+inline size_t elem_bytes(int dt) { return dt == DT_F32 ? 4 : 2; }
+inline bool is_elem(int dt) { return dt == DT_F32 || dt == DT_F16 || dt == DT_BF16; }
+
+// element i of a row of type dt; the type is the same for a whole launch, so the branch is uniform
+__device__ __forceinline__ float load_elem(const void *p, int dt, long long i) {
+    if (dt == DT_F32) return ((const float *)p)[i];
+    if (dt == DT_F16) return (float)((const half_t *)p)[i];
+    return (float)((const bf16_t *)p)[i];
+}
+__device__ __forceinline__ void store_elem(void *p, int dt, long long i, float v) {
+    if (dt == DT_F32) ((float *)p)[i] = v;
+    else if (dt == DT_F16) ((half_t *)p)[i] = (half_t)v;
+    else ((bf16_t *)p)[i] = (bf16_t)v;
+}
+
+// rows of `width` bytes, `ld` bytes apart, in samples `bs` bytes apart
+struct Window {
+    const void *p;
+    unsigned long long width, ld, rows, bs, samples;
+    unsigned long long end() const { return (unsigned long long)p + (samples - 1) * bs + (rows - 1) * ld + width; }
+};
+inline Window window(const void *p, size_t elem, unsigned long long width, unsigned long long ld,
+                     unsigned long long rows, unsigned long long bs = 0, unsigned long long samples = 1) {
+    return Window{p, width * elem, ld * elem, rows, bs * elem, samples};
+}
+// Whether two windows may share bytes. Apart from each other, or columns of the same rows (equal row strides, sample
+// strides whole rows, and column ranges that do not meet): they do not.
+inline bool windows_meet(const Window &a, const Window &b) {
+    const unsigned long long pa = (unsigned long long)a.p, pb = (unsigned long long)b.p;
+    if (pa >= b.end() || pb >= a.end()) return false;
+    if (a.ld != b.ld || a.bs % a.ld || b.bs % a.ld) return true;
+    const unsigned long long d = (pb >= pa ? pb - pa : a.ld - (pa - pb) % a.ld) % a.ld;   // b's first column after a's
+    return !(d >= a.width && d + b.width <= a.ld);
+}
+
+} // namespace tsn

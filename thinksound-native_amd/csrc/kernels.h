@@ -467,4 +467,49 @@ int launch_rms_head(float *x, const float *w, int rows, int nh, int ld, int hd, 
 int launch_rope_pairs(float *x, const int32_t *pos, int rows, int nh, int ld, int hd, int col_off,
                       int row_off, float fscale, float base, hipStream_t st);
 
+/* ------------------------------------------------------------------ block operators (blockops.hip, diffattn.hip) */
+// The fields of include/tsn.h's specs and the call's pointers. The *_check functions refuse what the kernels do not
+// take and fill in the packed strides; launching reads checked arguments.
+struct RopeAxesArgs {
+    int dt;
+    uint32_t rows, nh, hd, ldx, ldy, pos_rows, n_axes, dim[4];
+    float base[4], fscale[4];
+    int half_split, inverse;
+    const void *x;
+    const int32_t *pos;
+    void *y;
+};
+struct DiffAttnArgs {
+    int dt;
+    uint32_t B, Sq, Sk, nh, nkv, hd, ldq, ldk, ldv, ldo;
+    uint64_t bsq, bsk, bsv, bso;
+    uint32_t lam_heads;
+    int causal;
+    float scale, lambda_init, eps;
+    const void *q, *k, *v;
+    const float *lam, *norm_w;
+    const int32_t *q_len, *kv_len;
+    void *out;
+};
+enum { NORM_NONE = 0, NORM_RMS = 1, NORM_LN = 2 };
+struct GateNormArgs {
+    uint32_t rows, H;
+    int xdt, fdt, ydt, post, pre;
+    uint32_t ldx, ldf, ldo, ldy;
+    float x_scale, f_scale;
+    uint32_t chunks, mod_rows;
+    int gate, shift, scale;
+    float post_eps, pre_eps;
+    const void *x, *f;
+    const float *mod, *post_w, *post_b, *pre_w, *pre_b;
+    void *x_out, *y;
+};
+int rope_axes_check(RopeAxesArgs &a);
+int diff_attention_check(DiffAttnArgs &a);
+int gate_add_norm_check(GateNormArgs &a);
+int launch_rope_axes(const RopeAxesArgs &a, hipStream_t st);
+// ws: partial results of a split over the keys (ws_bytes of it), on the stream's own runtime
+int launch_diff_attention(const DiffAttnArgs &a, float *ws, size_t ws_bytes, hipStream_t st);
+int launch_gate_add_norm(const GateNormArgs &a, hipStream_t st);
+
 } // namespace tsn

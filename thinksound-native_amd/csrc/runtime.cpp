@@ -451,6 +451,19 @@ int Runtime::attention(const float *qkv, float *out, uint32_t S, uint32_t nh, ui
     return launch_attention(a, dev.stream());
 }
 
+int Runtime::rope_axes(const RopeAxesArgs &a) {
+    TSN_TRY(dev.make_current());
+    return launch_rope_axes(a, dev.stream());
+}
+int Runtime::diff_attention(const DiffAttnArgs &a) {
+    TSN_TRY(dev.make_current());
+    return launch_diff_attention(a, split_ws(), split_ws_bytes(), dev.stream());
+}
+int Runtime::gate_add_norm(const GateNormArgs &a) {
+    TSN_TRY(dev.make_current());
+    return launch_gate_add_norm(a, dev.stream());
+}
+
 int Runtime::probe_peaks(double *mfma_tflops, double *hbm_gbs) {
     TSN_REQUIRE(mfma_tflops && hbm_gbs, "probe: null output");
     TSN_TRY(dev.make_current());

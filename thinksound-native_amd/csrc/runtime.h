@@ -130,6 +130,10 @@ public:
                    uint32_t col_off, uint32_t row_off, float fscale, float base);
     int attention(const float *qkv, float *out, uint32_t S, uint32_t nh, uint32_t hd, uint32_t ld,
                   uint32_t ldo, uint32_t q_off, uint32_t k_off, uint32_t v_off, uint32_t o_off, float scale);
+    // block operators without a reference counterpart; arguments checked (rope_axes_check and its like)
+    int rope_axes(const RopeAxesArgs &a);
+    int diff_attention(const DiffAttnArgs &a);
+    int gate_add_norm(const GateNormArgs &a);
 
     // calibration: achievable dense f16 MFMA TFLOP/s (one workgroup of 8 waves per CU) and
     // device-to-device copy GB/s (read + write of a 1 GiB buffer), timed with events on the stream
