@@ -222,7 +222,7 @@ def run(st):
             rt.gate_add_norm(st.plan, i["x"], i["f"], i["mod"], o["x"], o["y"], i.get("post_w"), i.get("post_b"),
                              i.get("pre_w"), i.get("pre_b"))
         else:
-            rt.diff_attention(st.plan, i["q"], i["k"], i["v"], i["lam"], i["w"], o["o"], i["ql"], i["kl"])
+            rt.diff_attention(st.plan, i["q"], i["k"], i["v"], i["lam"], i["w"], i["ql"], i["kl"], o["o"])
         return st.out
     return {"rope": _plain_rope, "norm": _plain_norm, "attn": _plain_attn}[st.case["op"]](st)
 
