@@ -147,8 +147,9 @@ int tsn_attention(tsn_runtime *rt, const float *qkv, float *out, uint32_t S, uin
                   uint32_t ldo, uint32_t q_off, uint32_t k_off, uint32_t v_off, uint32_t o_off, float scale);
 
 /* ---------------- transformer block operators beside the launchers above (no reference counterpart) ----------------
- * Inference forms, all on the runtime's stream, none allocating device memory. Each reads its spec (host memory)
- * before it returns. Argument errors are found before anything is launched. */
+ * Inference forms, all on the runtime's stream. Each reads its spec (host memory) before it returns. Argument errors
+ * are found before anything is launched. Only tsn_diff_attention uses device memory of its own: the runtime's
+ * grow-on-demand scratch (see there). */
 
 /* Rotary positions with several axes (time, height, width): tsn_rope_pairs for clip rows cut from frames. Pair i of
  * axis a of every head of row r turns by
@@ -182,8 +183,9 @@ int tsn_rope_axes(tsn_runtime *rt, const tsn_rope_axes_spec *spec, const void *x
  * from kv_len on may hold anything, infinities and NaN among it; those before are finite.
  * f16 or bf16 in and out; scores, softmax statistics and sums in f32, probabilities rounded to the inputs' type for
  * the product with v. 16-byte aligned pointers and strides of a multiple of 8 elements run on MFMA, others a plain
- * kernel. out must not overlap an input. Partial results of long keys over few rows go to the runtime's 32 MiB
- * workspace and are joined in a fixed order: same bits on every run. */
+ * kernel. out must not overlap an input. Where the rows alone do not fill the device, or their last round of workgroups
+ * would be far from full, keys are shared out among workgroups: partial results go to the runtime's grow-on-demand
+ * scratch and are joined in the order of the keys: same bits on every run. */
 typedef struct {
     int dtype;                    /* q, k, v and out: TSN_F16 or TSN_BF16 */
     uint32_t B, Sq, Sk;           /* samples, rows and keys of each */

@@ -496,19 +496,25 @@ def test_diff_attention_far_rows(tsn, rt):
     big.free()
 
 
-def test_block_operators_allocate_nothing(tsn):
-    """none of the calls takes device memory: the runtime's allocations are as before"""
+def test_block_operators_allocations(tsn):
+    """rope_axes and gate_add_norm take no device memory, diff_attention the runtime's scratch once: a second call of the
+    same or a smaller size allocates nothing"""
     r = rng(9)
     with tsn.Runtime(0) as rt2:
         q, k = rt2.array(enc(r.standard_normal((1, 4, 256)), F16)), rt2.array(enc(r.standard_normal((1, 9000, 256)), F16))
         lam, o = rt2.array(np.zeros((1, 4, 64), np.float32)), rt2.empty((1, 4, 256), np.float16)
         pos, y = rt2.array(np.zeros((4, 1), np.int32)), rt2.empty((4, 256), np.float16)
         before = rt2.alloc_stats()
-        rt2.diff_attention(tsn.diff_attn_spec(F16, 1, 4, 9000, 2, 2, 64), q, k, k, lam, None, None, None, o)
         rt2.rope_axes(tsn.rope_axes_spec(F16, 4, 4, 64, (64,), (1e4,)), q, pos, y)
         rt2.gate_add_norm(tsn.gate_norm_spec(4, 256, F16, F16, F16), q, y, None, q, y)
-        rt2.sync()
         assert rt2.alloc_stats() == before
+        rt2.diff_attention(tsn.diff_attn_spec(F16, 1, 4, 9000, 2, 2, 64), q, k, k, lam, None, None, None, o)
+        once = rt2.alloc_stats()
+        assert once[0] <= before[0] + 1
+        for Sk in (9000, 5000):
+            rt2.diff_attention(tsn.diff_attn_spec(F16, 1, 4, Sk, 2, 2, 64), q, k, k, lam, None, None, None, o)
+        rt2.sync()
+        assert rt2.alloc_stats() == once
 
 
 def test_two_runtimes_at_once(tsn, rt):

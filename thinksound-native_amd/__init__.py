@@ -994,39 +994,34 @@ class Runtime:
     # --- block operators: device arrays, and a spec made once (rope_axes_spec, diff_attn_spec, gate_norm_spec) ---
     def rope_axes(self, spec, x, pos, y):
         """multi-axis rotary positions of the heads in x's rows, to y (which may be x)"""
-        n = spec.rows and spec.nh * spec.hd
-        size = 4 if spec.dtype == F32 else 2
-        _need("rope_axes: x", x, _span(spec.rows, spec.ldx or n, n), size)
-        _need("rope_axes: pos", pos, (spec.pos_rows or spec.rows) * spec.n_axes)
-        _need("rope_axes: y", y, _span(spec.rows, spec.ldy or n, n), size)
+        rows, size = spec.rows, 4 if spec.dtype == F32 else 2
+        n = spec.nh * spec.hd
+        _hold("rope_axes", (("x", x, _span(rows, spec.ldx or n, n) * size),
+                            ("pos", pos, (spec.pos_rows or rows) * spec.n_axes * 4),
+                            ("y", y, _span(rows, spec.ldy or n, n) * size)))
         call("tsn_rope_axes", self.h, spec, x.p, pos.p, y.p)
 
     def diff_attention(self, spec, q, k, v, lam, norm_w, q_len, kv_len, out):
         """differential attention; norm_w, q_len and kv_len may be None"""
-        s = spec
-        wq, wk = 2 * s.nh * s.hd, 2 * s.nkv * s.hd
-        _need("diff_attention: q", q, _span3(s.B, s.Sq, s.ldq or wq, s.bsq, wq), 2)
-        _need("diff_attention: k", k, _span3(s.B, s.Sk, s.ldk or wk, s.bsk, wk), 2)
-        _need("diff_attention: v", v, _span3(s.B, s.Sk, s.ldv or wk, s.bsv, wk), 2)
-        _need("diff_attention: out", out, _span3(s.B, s.Sq, s.ldo or wq, s.bso, wq), 2)
-        _need("diff_attention: lam", lam, 4 * s.lam_heads * s.hd)
-        _need("diff_attention: norm_w", norm_w, 2 * s.hd, optional=True)
-        _need("diff_attention: q_len", q_len, s.B, optional=True)
-        _need("diff_attention: kv_len", kv_len, s.B, optional=True)
-        call("tsn_diff_attention", self.h, s, q.p, k.p, v.p, lam.p, _p(norm_w), _p(q_len), _p(kv_len), out.p)
+        B, Sq, Sk, hd = spec.B, spec.Sq, spec.Sk, spec.hd
+        wq, wk = 2 * spec.nh * hd, 2 * spec.nkv * hd
+        _hold("diff_attention", (("q", q, 2 * _span3(B, Sq, spec.ldq or wq, spec.bsq, wq)),
+                                 ("k", k, 2 * _span3(B, Sk, spec.ldk or wk, spec.bsk, wk)),
+                                 ("v", v, 2 * _span3(B, Sk, spec.ldv or wk, spec.bsv, wk)),
+                                 ("out", out, 2 * _span3(B, Sq, spec.ldo or wq, spec.bso, wq)),
+                                 ("lam", lam, 16 * spec.lam_heads * hd)),
+              (("norm_w", norm_w, 8 * hd), ("q_len", q_len, 4 * B), ("kv_len", kv_len, 4 * B)))
+        call("tsn_diff_attention", self.h, spec, q.p, k.p, v.p, lam.p, _p(norm_w), _p(q_len), _p(kv_len), out.p)
 
     def gate_add_norm(self, spec, x, f, mod, x_out, y, post_w=None, post_b=None, pre_w=None, pre_b=None):
         """x_out = x_scale*x + f_scale*gate*post(f), y = pre(x_out)*(1 + scale) + shift; y and mod may be None"""
-        s = spec
-        size = lambda dt: 4 if dt == F32 else 2  # noqa: E731
-        _need("gate_add_norm: x", x, _span(s.rows, s.ldx or s.H, s.H), size(s.x_dtype))
-        _need("gate_add_norm: f", f, _span(s.rows, s.ldf or s.H, s.H), size(s.f_dtype))
-        _need("gate_add_norm: x_out", x_out, _span(s.rows, s.ldo or s.H, s.H), size(s.x_dtype))
-        _need("gate_add_norm: y", y, _span(s.rows, s.ldy or s.H, s.H), size(s.y_dtype), optional=True)
-        _need("gate_add_norm: mod", mod, (-(-s.rows // s.mod_rows) if s.mod_rows else 1) * s.chunks * s.H, optional=True)
-        for name, w in (("post_w", post_w), ("post_b", post_b), ("pre_w", pre_w), ("pre_b", pre_b)):
-            _need("gate_add_norm: " + name, w, s.H, optional=True)
-        call("tsn_gate_add_norm", self.h, s, x.p, f.p, _p(mod), _p(post_w), _p(post_b), _p(pre_w), _p(pre_b), x_out.p,
+        rows, H, m = spec.rows, spec.H, spec.mod_rows
+        sx, sf, sy = (4 if dt == F32 else 2 for dt in (spec.x_dtype, spec.f_dtype, spec.y_dtype))
+        _hold("gate_add_norm", (("x", x, _span(rows, spec.ldx or H, H) * sx), ("f", f, _span(rows, spec.ldf or H, H) * sf),
+                                ("x_out", x_out, _span(rows, spec.ldo or H, H) * sx)),
+              (("y", y, _span(rows, spec.ldy or H, H) * sy), ("mod", mod, (-(-rows // m) if m else 1) * spec.chunks * H * 4),
+               ("post_w", post_w, 4 * H), ("post_b", post_b, 4 * H), ("pre_w", pre_w, 4 * H), ("pre_b", pre_b, 4 * H)))
+        call("tsn_gate_add_norm", self.h, spec, x.p, f.p, _p(mod), _p(post_w), _p(post_b), _p(pre_w), _p(pre_b), x_out.p,
              _p(y))
 
     def silu(self, x, n):
@@ -1066,6 +1061,16 @@ def _need(what, arr, numel, itemsize=4, optional=False):
         raise TypeError("%s: expected a DeviceArray, got %r" % (what, type(arr)))
     if have < numel * itemsize:
         raise ValueError("%s: %d bytes needed, the array holds %d" % (what, numel * itemsize, have))
+
+
+def _hold(what, arrays, optional=()):
+    """_need of several (name, array, bytes); the optional ones may be None"""
+    for name, arr, nbytes in arrays:
+        if arr is None or getattr(arr, "nbytes", -1) < nbytes or not hasattr(arr, "p"):
+            _need("%s: %s" % (what, name), arr, nbytes, 1)
+    for name, arr, nbytes in optional:
+        if arr is not None and (getattr(arr, "nbytes", -1) < nbytes or not hasattr(arr, "p")):
+            _need("%s: %s" % (what, name), arr, nbytes, 1)
 
 
 def _p(arr):

@@ -4,6 +4,8 @@
 // One pass over the keys: each map keeps its running maximum, sum and product with V (the online
 // softmax), and the two are joined once both sums are known.
 #include <math.h>
+#include <stdio.h>
+#include <stdlib.h>
 
 #include "kernels.h"
 
@@ -122,16 +124,27 @@ __global__ __launch_bounds__(256) void diff_attn_any_kernel(const DiffAttnArgs a
 typedef __attribute__((address_space(3))) char lds_char;
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) i32x4 lds_i32x4;
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-__device__ __forceinline__ floatx16 mfma32(s16x8 a, s16x8 b, floatx16 c, half_t) {
+__device__ __forceinline__ floatx16 mfma32(i32x4 a, i32x4 b, floatx16 c, half_t) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ floatx16 mfma32(s16x8 a, s16x8 b, floatx16 c, bf16_t) {
+__device__ __forceinline__ floatx16 mfma32(i32x4 a, i32x4 b, floatx16 c, bf16_t) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// two values rounded to nearest even, in one register
+template <typename T> struct Pair;
+template <> struct Pair<half_t> { typedef half2_t type; };
+template <> struct Pair<bf16_t> { typedef bf16x2 type; };
+template <typename T>
+__device__ __forceinline__ int pack2(float a, float b) {
+    return __builtin_bit_cast(int, __builtin_convertvector((floatx2{a, b}), typename Pair<T>::type));
 }
 __device__ __forceinline__ floatx16 zero16() {
     return floatx16{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -146,16 +159,19 @@ __device__ __forceinline__ float pair_sum(float v) {
     return __uint_as_float(p[0]) + __uint_as_float(p[1]);
 }
 
-// 16 bytes a lane, global -> LDS slot (lane) of the 1 KB block at lds; offsets past the resource's 2^31 bytes read as
-// zero. Ordered by explicit vmcnt waits; s_nop 0 covers the M0 -> LDS-DMA hazard.
-__device__ __forceinline__ void dma16(const void *base, unsigned voff, const lds_char *lds) {
-    const unsigned l = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long)lds);
+// A buffer of `bytes` (at most 2^30) bytes: loads from behind its end read as zero
+__device__ __forceinline__ i32x4 buffer(const void *base, unsigned bytes) {
     const unsigned long long p = (unsigned long long)base;
-    const i32x4 rs = i32x4{(int)__builtin_amdgcn_readfirstlane((unsigned)p),
-                           (int)(__builtin_amdgcn_readfirstlane((unsigned)(p >> 32)) & 0xFFFF), 0x7FFFFFFF, 0x00020000};
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+    return i32x4{(int)__builtin_amdgcn_readfirstlane((unsigned)p), (int)(__builtin_amdgcn_readfirstlane((unsigned)(p >> 32)) & 0xFFFF),
+                 (int)__builtin_amdgcn_readfirstlane(bytes), 0x00020000};
+}
+// 16 bytes a lane at voff + soff, global -> LDS slot (lane) of the 1 KB block at address lds. Ordered by explicit vmcnt
+// waits; s_nop 0 covers the M0 -> LDS-DMA hazard.
+__device__ __forceinline__ void dma16(i32x4 rs, unsigned voff, unsigned soff, unsigned lds) {
+    const unsigned l = __builtin_amdgcn_readfirstlane(lds), so = __builtin_amdgcn_readfirstlane(soff);
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
                  :
-                 : "v"(voff), "s"(rs), "s"(l)
+                 : "v"(voff), "s"(rs), "s"(so), "s"(l)
                  : "memory");
 }
 template <int N>
@@ -193,99 +209,128 @@ __device__ __forceinline__ int key_of(int i) { return 16 * (i >> 4) + 8 * ((i >>
 // What a wave holds of its 32 rows: queries, running reference (log2 units), each lane's share of the sums, products
 template <int HD>
 struct Rows {
-    s16x8 q[2][Lay<HD>::KS];
+    i32x4 q[2][Lay<HD>::KS];
     float m[2], l[2];
     floatx16 o[2][Lay<HD>::DT];
     int lim;   // keys that the lane's row sees
 };
 
-// NB blocks of 1 KB of one operand: rows row0 + blk*RPB.. of the tile that starts at `base`, into the tile at lds;
-// rows from `valid` on read as zero
-template <int HD, bool V>
-__device__ __forceinline__ void load_block(const char *base, unsigned ld_bytes, int blk, int valid, const lds_char *tile, int lane) {
+// The lane's share of a tile's loads. Block i of a wave's holds rows r0 + i*RPB.. of the tile; row r's chunk c goes to
+// slot c ^ swizzle(r). The K swizzle of block i is that of block 0 ^ 4i, the V swizzle the same for all.
+template <int HD, int NB>
+struct Loads {
+    unsigned k[NB], v;   // byte offsets in the tile: K for each block, V (blocks RPB rows apart)
+};
+template <int HD, int NB>
+__device__ __forceinline__ Loads<HD, NB> lane_loads(int row0, unsigned ldk, unsigned ldv, int lane) {
     using L = Lay<HD>;
-    const int r = blk * L::RPB + lane / L::CPR;
-    const int c = (lane % L::CPR) ^ (V ? L::vsw(r) : L::ksw(r));
-    dma16(base, r < valid ? (unsigned)r * ld_bytes + c * 16 : 0x80000000u, tile + blk * 1024);
+    Loads<HD, NB> o;
+    const int r = row0 + lane / L::CPR, c = lane % L::CPR;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) o.k[i] = (unsigned)r * ldk + ((c ^ L::ksw(r + i * L::RPB)) << 4);
+    o.v = (unsigned)r * ldv + ((c ^ L::vsw(r)) << 4);
+    return o;
+}
+// the wave's NB blocks of K to lds, NB of V to lds + v_off; `rows` of the tile are there, the others read as zero
+template <int HD, int NB>
+__device__ __forceinline__ void load_tile(const Loads<HD, NB> &o, const char *kt, const char *vt, unsigned ldk, unsigned ldv, int rows,
+                                          unsigned lds, unsigned v_off) {
+    using L = Lay<HD>;
+    const int n = rows - 1;
+    const i32x4 rk = buffer(kt, n < 0 ? 0u : (unsigned)n * ldk + L::ROW), rv = buffer(vt, n < 0 ? 0u : (unsigned)n * ldv + L::ROW);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) dma16(rk, o.k[i], i * L::RPB * ldk, lds + i * 1024);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) dma16(rv, o.v, i * L::RPB * ldv, lds + v_off + i * 1024);
 }
 
-// Online softmax and products of 32 keys, key 0 of them at k0, K and V rows at the LDS tiles sK, sV. The reference m
-// moves only when a score passes it by more than 2^8 (then O and the sums are rescaled): probabilities stay below 2^8,
-// inside f16, and most steps skip it.
+// LDS addresses of the lane's part of a tile of 32 rows: K row key_of(lane & 31), V row 8*(lane>>5) + (lane&15)/4. Other
+// chunks are reached by ^ (bits 4 to 7), other rows, blocks and stages by +: they do not meet.
+template <int HD>
+__device__ __forceinline__ unsigned k_lane(int lane) {
+    const int r = key_of(lane & 31);
+    return r * Lay<HD>::ROW + (((lane >> 5) ^ Lay<HD>::ksw(r)) << 4);
+}
+template <int HD>
+__device__ __forceinline__ unsigned v_lane(int lane) {
+    const int r = 8 * (lane >> 5) + ((lane & 15) >> 2);
+    return r * Lay<HD>::ROW + (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ Lay<HD>::vsw(r)) << 4) + (lane & 1) * 8;
+}
+// S^T of both maps for 32 keys, k = k_lane + the K tile's address
 template <typename T, int HD>
-__device__ __forceinline__ void step32(Rows<HD> &w, const lds_char *sK, const lds_char *sV, int k0, bool mask, float c, int lane) {
+__device__ __forceinline__ void scores(const Rows<HD> &w, unsigned k, floatx16 (&s)[2]) {
     using L = Lay<HD>;
-    const int g = lane >> 5;
-    const int kr = key_of(lane & 31);
-    floatx16 s[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         s[j] = zero16();
 #pragma unroll
-        for (int ks = 0; ks < L::KS; ++ks) {
-            const int slot = (j * (HD / 8) + ks * 2 + g) ^ L::ksw(kr);
-            const s16x8 kf = *(const __attribute__((address_space(3))) s16x8 *)(sK + kr * L::ROW + slot * 16);
-            s[j] = mfma32(kf, w.q[j][ks], s[j], T());
-        }
+        for (int ks = 0; ks < L::KS; ++ks)
+            s[j] = mfma32(*(lds_i32x4 *)(k ^ ((j * (HD / 8) + ks * 2) << 4)), w.q[j][ks], s[j], T());
     }
-    if (mask) {   // the same for the whole wave
-        const int left = w.lim - k0 - 8 * g;
+}
+// scores of keys that the lane's row does not see: key 0 of the 32 at k0
+template <int HD>
+__device__ __forceinline__ void mask_scores(const Rows<HD> &w, floatx16 (&s)[2], int k0, int lane) {
+    const int left = w.lim - k0 - 8 * (lane >> 5);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-            if (16 * (r >> 3) + (r & 7) >= left) s[0][r] = s[1][r] = -INFINITY;
-    }
-    float top[2];
+    for (int r = 0; r < 16; ++r)
+        if (16 * (r >> 3) + (r & 7) >= left) s[0][r] = s[1][r] = -INFINITY;
+}
+// Probabilities of 32 keys. The reference m moves only when a score passes it by more than 2^8: probabilities stay
+// below 2^8, inside f16, and most steps leave O as it is. Returns whether any lane's moved; al: by what O has to be
+// scaled before these probabilities' product is added.
+template <typename T, int HD>
+__device__ __forceinline__ bool probs(Rows<HD> &w, const floatx16 (&s)[2], i32x4 (&p)[2][2], float (&al)[2], float c) {
+    bool moved = false;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         float t = fmaxf(fmaxf(s[j][0], s[j][1]), s[j][2]);
 #pragma unroll
         for (int r = 3; r < 15; r += 2) t = fmaxf(fmaxf(t, s[j][r]), s[j][r + 1]);
-        top[j] = pair_max(fmaxf(t, s[j][15])) * c;
-    }
-    const bool up0 = top[0] > w.m[0] + 8.0f, up1 = top[1] > w.m[1] + 8.0f;
-    if (__builtin_amdgcn_ballot_w64(up0 || up1) != 0) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float mn = (j ? up1 : up0) ? top[j] : w.m[j];
-            const float al = __builtin_amdgcn_exp2f(w.m[j] - mn);
-            w.m[j] = mn;
-            w.l[j] *= al;
-#pragma unroll
-            for (int d = 0; d < L::DT; ++d) w.o[j][d] *= al;
-        }
-    }
-    s16x8 p[2][2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
+        t = pair_max(fmaxf(t, s[j][15])) * c;
+        const bool up = t > w.m[j] + 8.0f;
+        const float mn = up ? t : w.m[j];
+        al[j] = __builtin_amdgcn_exp2f(w.m[j] - mn);
+        w.m[j] = mn;
+        moved |= up;
         float sum = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], c, -w.m[j]));
-            sum += e;
-            p[j][r >> 3][r & 7] = __builtin_bit_cast(short, (T)e);
+        for (int r = 0; r < 16; r += 2) {
+            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], c, -mn));
+            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r + 1], c, -mn));
+            sum += e0;
+            sum += e1;
+            p[j][r >> 3][(r & 7) >> 1] = pack2<T>(e0, e1);
         }
-        w.l[j] += sum;
+        w.l[j] = __builtin_fmaf(w.l[j], al[j], sum);
     }
-    // A row = column 32d + (lane & 31) of V, keys 16*h + 8g + 0..7 by two transposing reads of four
-    const int vr = 8 * g + ((lane & 15) >> 2);
-    const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    return __builtin_amdgcn_ballot_w64(moved) != 0;
+}
+template <int HD>
+__device__ __forceinline__ void rescale(Rows<HD> &w, const float (&al)[2]) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int d = 0; d < L::DT; ++d) {
-            s16x4 v[2];
+        for (int d = 0; d < Lay<HD>::DT; ++d) w.o[j][d] *= al[j];
+}
+// O^T += V^T P^T for 32 keys, v = v_lane + the V tile's address: A row = column 32d + (lane & 31) of V, keys
+// 16h + 8*(lane>>5) + 0..7 by two transposing reads of four
+template <typename T, int HD>
+__device__ __forceinline__ void product(Rows<HD> &w, unsigned v, const i32x4 (&p)[2][2]) {
+    using L = Lay<HD>;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int r = 16 * h + vr + 4 * e;
-                v[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (lds_s16x4 *)(sV + r * L::ROW + ((4 * d + vc) ^ L::vsw(r)) * 16 + (lane & 1) * 8));
-            }
-            const s16x8 vf = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    for (int d = 0; d < L::DT; ++d) {
+        const unsigned vd = v ^ (d << 6);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int2 lo = __builtin_bit_cast(int2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vd + 16 * h * L::ROW)));
+            const int2 hi = __builtin_bit_cast(int2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vd + (16 * h + 4) * L::ROW)));
+            const i32x4 vf = i32x4{lo.x, lo.y, hi.x, hi.y};
             w.o[0][d] = mfma32(vf, p[0][h], w.o[0][d], T());
             w.o[1][d] = mfma32(vf, p[1][h], w.o[1][d], T());
         }
+    }
 }
-
 // Row x of a key/value head: its query and head within the group
 struct RowOf {
     int qi, hg;
@@ -305,8 +350,8 @@ __device__ __forceinline__ void load_rows(Rows<HD> &w, const DiffAttnArgs &a, in
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int ks = 0; ks < L::KS; ++ks) {
-            w.q[j][ks] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
-            if (in) w.q[j][ks] = *(const s16x8 *)(q + j * HD + ks * 16);
+            w.q[j][ks] = i32x4{0, 0, 0, 0};
+            if (in) w.q[j][ks] = *(const i32x4 *)(q + j * HD + ks * 16);
         }
         w.m[j] = -1e30f;
         w.l[j] = 0.0f;
@@ -327,89 +372,387 @@ __device__ __forceinline__ float row_lambda(const DiffAttnArgs &a, int g, int G,
     return lam;
 }
 
-// Many rows: 128 rows of one key/value head a workgroup, 32 a wave; the four waves share tiles of 64 keys, two stages
-// in LDS, the next tile loaded while this one is multiplied.
-template <typename T, int HD>
-__global__ __launch_bounds__(256, HD == 64 ? 1 : 2) void diff_attn_rows_kernel(const DiffAttnArgs a, int ntile) {
+// How a launch's work is cut. A tile is 32*RW rows of one key/value head of one sample, its keys are units of KB. The
+// first `full` tiles have a workgroup each. The units of the others, one after the other, are shared out evenly among
+// `shared` workgroups; their pieces of tiles go to the workspace and are joined by diff_attn_join_kernel. A piece's place
+// there is its workgroup's number plus its tile's: both only grow along the units, and one of them does at every cut.
+struct DiffPlan {
+    int ntile;          // tiles of a key/value head
+    int tiles, units;   // of all heads and samples; of a tile (by Sk)
+    int full, shared;
+    int by_len;         // full = 0 and lengths are given: the units are counted by them
+    float *o;           // [piece][row of the tile][map][2 HD]: products with V, not divided
+    float4 *st;         // [piece][row of the tile]: reference and sum of each map
+};
+struct Share {   // shared workgroup p's units begin at p*q + min(p, r)
+    unsigned q, r;
+    __device__ __forceinline__ unsigned begin(unsigned p) const { return p * q + min(p, r); }
+    __device__ __forceinline__ unsigned holder(unsigned u) const { return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q; }
+};
+// A unit's tile: sample, place among the sample's tiles (of which each head has `heads`), first unit, units of a tile
+struct Spot {
+    int b, tile, heads;
+    unsigned first, n;
+};
+// By the lengths: a wave looks at 64 samples at a time. Of sample b, nkv * tiles * n units.
+template <int RW, int KB>
+struct ByLen {
+    __device__ static __forceinline__ void sample(const DiffAttnArgs &a, int b, int &tiles, unsigned &n) {
+        const int G = (int)(a.nh / a.nkv);
+        tiles = (int)(((unsigned)q_rows(a, b) * G + 32 * RW - 1) / (32 * RW));
+        n = (unsigned)max(1, (kv_rows(a, b) + KB - 1) / KB);
+    }
+    // units up to and with the lane's sample, of the 64 from b0 on
+    __device__ static __forceinline__ unsigned scan(const DiffAttnArgs &a, int b0, int lane, unsigned &own) {
+        int tiles = 0;
+        unsigned n = 0;
+        if (b0 + lane < (int)a.B) sample(a, b0 + lane, tiles, n);
+        own = a.nkv * tiles * n;
+        unsigned v = own;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const unsigned w = __shfl_up(v, d);
+            if (lane >= d) v += w;
+        }
+        return v;
+    }
+    __device__ static __forceinline__ unsigned total(const DiffAttnArgs &a, int lane) {
+        unsigned t = 0, own;
+        for (int b0 = 0; b0 < (int)a.B; b0 += 64) t += __builtin_amdgcn_readlane(scan(a, b0, lane, own), 63);
+        return t;
+    }
+    __device__ static __forceinline__ Spot find(const DiffAttnArgs &a, unsigned u, int lane) {
+        unsigned before = 0;
+        for (int b0 = 0; b0 < (int)a.B; b0 += 64) {
+            unsigned own;
+            const unsigned upto = scan(a, b0, lane, own), all = __builtin_amdgcn_readlane(upto, 63);
+            if (u < before + all) {
+                const int i = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(before + upto > u)) - 1;
+                Spot s;
+                s.b = b0 + i;
+                const unsigned start = before + __builtin_amdgcn_readlane(upto - own, i);
+                sample(a, s.b, s.heads, s.n);
+                s.tile = (int)((u - start) / s.n);
+                s.first = start + s.tile * s.n;
+                return s;
+            }
+            before += all;
+        }
+        return Spot{};   // u is below the total: not reached
+    }
+};
+
+// One tile or piece of one: 32 rows a wave, RW waves side by side; KW waves share the rows of one and take every KW-th
+// block of 32 keys, and are merged at the end through LDS. All four read the same K and V tiles, two stages in LDS: the
+// next is loaded while one is worked on. RW = 4: two workgroups a CU, one's matrix products cover the other's softmax.
+template <typename T, int HD, int RW, int KW>
+struct Attn {
     using L = Lay<HD>;
-    constexpr int KB = 64, OP = KB * L::ROW, STAGE = 2 * OP;
-    __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
-    const lds_char *lds = (const lds_char *)smem;
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const unsigned wg = xcd_remap(blockIdx.x, gridDim.x);
-    const unsigned bg = wg / (unsigned)ntile;
-    const int tile = a.causal ? ntile - 1 - (int)(wg - bg * ntile) : (int)(wg - bg * ntile);   // causal: long rows first
-    const int b = (int)(bg / a.nkv), g = (int)(bg - (unsigned)b * a.nkv), G = (int)(a.nh / a.nkv);
-    const int nq = q_rows(a, b), nk = kv_rows(a, b);
-    const int x0 = tile * 128;
-    if (x0 / G >= nq) return;   // the whole workgroup: no row of it is left
-    const int x = x0 + wave * 32 + (lane & 31);
-    Rows<HD> w;
-    load_rows<T, HD>(w, a, b, g, G, x, nq, nk, lane);
-    // keys that any row of the workgroup, any row of the wave, and every row of the wave sees
-    auto limit = [&](int xr) {
-        const int qi = min(row_of(xr, G).qi, nq - 1);
-        return a.causal ? min(nk, max(0, qi + nk - nq + 1)) : nk;
-    };
-    const int keys = limit(x0 + 127), wkeys = limit(x0 + wave * 32 + 31), all = limit(x0 + wave * 32);
-    const char *kp = (const char *)((const T *)a.k + (long long)b * a.bsk + g * 2 * HD);
-    const char *vp = (const char *)((const T *)a.v + (long long)b * a.bsv + g * 2 * HD);
-    const unsigned ldk = a.ldk * 2, ldv = a.ldv * 2;
-    auto issue = [&](int t, int stage) {
-        const int k0 = t * KB;
-        const char *kt = kp + (long long)k0 * ldk, *vt = vp + (long long)k0 * ldv;
-        constexpr int PW = OP / 1024 / 4;   // 1 KB blocks of K, of V, a wave
+    static constexpr int NSUB = KW > 2 ? KW : 2;     // blocks of 32 keys in a unit
+    static constexpr int KB = 32 * NSUB;
+    static constexpr int OP = KB * L::ROW, STAGE = 2 * OP, SUB = 32 * L::ROW;
+    static constexpr int NB = OP / 1024 / 4;         // 1 KB blocks of K, of V, a wave and unit
+    static constexpr int NO = L::DT * 16;            // products of a lane and map
+    static constexpr int NQ = NO / KW;               // those that the lane has after the merge
+    static constexpr int STATS = KW > 1 ? 4 * 64 * 5 * 4 : 0;
+    static constexpr int LDS = 2 * STAGE + STATS;
+    static_assert(RW * KW == 4 && (KW == 1 || KW * 2 * NO * 256 <= 2 * STAGE), "four waves, whose products fit in the stages");
+
+    // Every wave leaves its products in LDS and takes values kw*NQ.. of all. Each lane's four are 16 bytes, lanes next to each other.
+    static __device__ __forceinline__ void merge(Rows<HD> &w, float (&o)[2][NQ], char *smem, int kw, int lane) {
+        float4 *all = (float4 *)smem + lane;
+        float4 *st = (float4 *)(smem + 2 * STAGE) + lane;
+        block_barrier();   // the key tiles have been read
 #pragma unroll
-        for (int i = 0; i < PW; ++i) load_block<HD, false>(kt, ldk, wave * PW + i, nk - k0, lds + stage * STAGE, lane);
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int i = 0; i < PW; ++i) load_block<HD, true>(vt, ldv, wave * PW + i, nk - k0, lds + stage * STAGE + OP, lane);
-    };
-    const float c = a.scale > 0.0f ? a.scale * LOG2E : 1e-30f;   // a scale of 0 must not meet a masked score's infinity
-    const int nt = (keys + KB - 1) / KB;
-    if (nt > 0) issue(0, 0);
-    for (int t = 0; t < nt; ++t) {
-        wait_vmcnt<0>();
+            for (int i = 0; i < NO; i += 4)
+                all[(kw * (NO / 2) + (j * NO + i) / 4) * 64] = make_float4(w.o[j][i >> 4][i & 15], w.o[j][i >> 4][(i & 15) + 1],
+                                                                           w.o[j][i >> 4][(i & 15) + 2], w.o[j][i >> 4][(i & 15) + 3]);
+        st[kw * 64] = make_float4(w.m[0], w.l[0], w.m[1], w.l[1]);
         block_barrier();
-        if (t + 1 < nt) issue(t + 1, (t + 1) & 1);
-        const lds_char *sK = lds + (t & 1) * STAGE, *sV = sK + OP;
+        float f[2][KW];
+        w.m[0] = w.m[1] = -1e30f;
+        w.l[0] = w.l[1] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KW; ++k) {
+            const float4 v = st[k * 64];
+            w.m[0] = fmaxf(w.m[0], v.x);
+            w.m[1] = fmaxf(w.m[1], v.z);
+        }
+#pragma unroll
+        for (int k = 0; k < KW; ++k) {
+            const float4 v = st[k * 64];
+            f[0][k] = __builtin_amdgcn_exp2f(v.x - w.m[0]);
+            f[1][k] = __builtin_amdgcn_exp2f(v.z - w.m[1]);
+            w.l[0] += v.y * f[0][k];
+            w.l[1] += v.w * f[1][k];
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < NQ; i += 4) {
+                float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int k = 0; k < KW; ++k) {
+                    const float4 v = all[(k * (NO / 2) + (j * NO + kw * NQ + i) / 4) * 64];
+                    t.x += v.x * f[j][k];
+                    t.y += v.y * f[j][k];
+                    t.z += v.z * f[j][k];
+                    t.w += v.w * f[j][k];
+                }
+                o[j][i] = t.x;
+                o[j][i + 1] = t.y;
+                o[j][i + 2] = t.z;
+                o[j][i + 3] = t.w;
+            }
+    }
+
+    // units u0 to u1 of tile `tile` of head g of sample b; a piece of it (to the workspace) or, piece < 0, all of it
+    static __device__ __forceinline__ void run(const DiffAttnArgs &a, const DiffPlan &pl, char *smem, int b, int g, int tile, int u0, int u1,
+                                               int piece) {
+        const unsigned lds = (unsigned)(unsigned long)(lds_char *)smem;
+        const int lane = threadIdx.x & 63;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int rw = wave % RW, kw = wave / RW;
+        const int G = (int)(a.nh / a.nkv);
+        const int nq = q_rows(a, b), nk = kv_rows(a, b);
+        const int x0 = tile * 32 * RW;
+        if (x0 / G >= nq) return;   // the whole workgroup: no row of the tile is there
+        const int x = x0 + rw * 32 + (lane & 31);
+        Rows<HD> w;
+        load_rows<T, HD>(w, a, b, g, G, x, nq, nk, lane);
+        // keys that any row of the tile and every row of the wave sees
+        auto limit = [&](int xr) {
+            const int qi = min(row_of(xr, G).qi, nq - 1);
+            return a.causal ? min(nk, max(0, qi + nk - nq + 1)) : nk;
+        };
+        const int keys = limit(x0 + 32 * RW - 1), all = limit(x0 + rw * 32);
+        const char *kp = (const char *)((const T *)a.k + (long long)b * a.bsk + g * 2 * HD);
+        const char *vp = (const char *)((const T *)a.v + (long long)b * a.bsv + g * 2 * HD);
+        const unsigned ldk = a.ldk * 2, ldv = a.ldv * 2;
+        const Loads<HD, NB> lo = lane_loads<HD, NB>(wave * NB * L::RPB, ldk, ldv, lane);
+        const unsigned kl = lds + k_lane<HD>(lane), vl = lds + OP + v_lane<HD>(lane);
+        auto issue = [&](int u) {
+            const long long k0 = (long long)u * KB;
+            load_tile<HD, NB>(lo, kp + k0 * ldk, vp + k0 * ldv, ldk, ldv, min(KB, nk - u * KB), lds + (u & 1) * STAGE + wave * NB * 1024, OP);
+        };
+        const float c = a.scale > 0.0f ? a.scale * LOG2E : 1e-30f;   // a scale of 0 must not meet a masked score's infinity
+        const int end = min(u1, (keys + KB - 1) / KB);
+        block_barrier();   // an earlier piece's LDS has been read
+        if (u0 < end) issue(u0);
+        const RowOf ro = row_of(x, G);
+        // values i of a lane are columns 32(i>>4) + 8((i&15)>>2) + 4*(lane>>5) + (i&3)
+        const int i0 = kw * NQ, col0 = 32 * (i0 >> 4) + 2 * (i0 & 15) + 4 * (lane >> 5);
+        float lam = 0.0f, nw[KW > 1 ? NQ : 1];
+        if constexpr (KW > 1) {   // few rows, where latency counts: loaded beside the first keys
+            if (piece < 0) {
+                lam = row_lambda(a, g, G, ro.hg, lane);
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) nw[i] = a.norm_w ? a.norm_w[col0 + 32 * (i >> 4) + 8 * ((i & 15) >> 2) + (i & 3)] : 1.0f;
+            }
+        }
+        for (int u = u0; u < end; ++u) {
+            wait_vmcnt<0>();
+            block_barrier();
+            if (u + 1 < end) issue(u + 1);
+            const unsigned at = (u & 1) * STAGE;
 #pragma unroll 1
-        for (int i = 0; i < KB / 32; ++i) {
-            const int k0 = t * KB + 32 * i;
-            if (k0 >= wkeys) break;
-            step32<T, HD>(w, sK + 32 * i * L::ROW, sV + 32 * i * L::ROW, k0, k0 + 32 > all, c, lane);
+            for (int i = 0; i < NSUB / KW; ++i) {
+                const int blk = i * KW + kw;
+                const int k0 = u * KB + 32 * blk;
+                floatx16 s[2];
+                i32x4 p[2][2];
+                float al[2];
+                scores<T, HD>(w, kl + at + blk * SUB, s);
+                if (k0 + 32 > all) mask_scores<HD>(w, s, k0, lane);
+                if (probs<T, HD>(w, s, p, al, c)) rescale<HD>(w, al);
+                product<T, HD>(w, vl + at + blk * SUB, p);
+            }
+        }
+        float o[2][NQ];
+        if constexpr (KW > 1) {
+            merge(w, o, smem, kw, lane);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) o[j][i] = w.o[j][i >> 4][i & 15];
+        }
+        const float l0 = pair_sum(w.l[0]), l1 = pair_sum(w.l[1]);
+        if (piece >= 0) {
+            if (ro.qi >= nq) return;
+            const long long row = (long long)piece * (32 * RW) + rw * 32 + (lane & 31);
+            if (lane < 32 && kw == 0) pl.st[row] = make_float4(w.m[0], l0, w.m[1], l1);
+            float *to = pl.o + row * (4 * HD) + col0;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < NQ; i += 4)
+                    *(float4 *)(to + j * 2 * HD + 32 * (i >> 4) + 2 * (i & 15)) = make_float4(o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]);
+            return;
+        }
+        if constexpr (KW == 1) lam = row_lambda(a, g, G, ro.hg, lane);
+        const float r0 = l0 > 0.0f ? 1.0f / l0 : 0.0f, r1 = l1 > 0.0f ? lam / l1 : 0.0f;
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            o[0][i] = o[0][i] * r0 - o[1][i] * r1;
+            ss += o[0][i] * o[0][i];
+        }
+        ss = pair_sum(ss);
+        if constexpr (KW > 1) {   // the row's squares over the waves, in their order
+            float *red = (float *)(smem + 2 * STAGE + 4 * 64 * 16) + lane;
+            red[kw * 64] = ss;
+            block_barrier();
+            ss = red[0];
+#pragma unroll
+            for (int k = 1; k < KW; ++k) ss += red[k * 64];
+        }
+        if (ro.qi >= nq) return;
+        if (a.norm_w) {
+            const float f = (1.0f - a.lambda_init) / sqrtf(ss / (float)(2 * HD) + a.eps);
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                if constexpr (KW > 1) o[0][i] = o[0][i] * f * nw[i];
+                else o[0][i] = o[0][i] * f * a.norm_w[col0 + 32 * (i >> 4) + 8 * ((i & 15) >> 2) + (i & 3)];
+            }
+        }
+        T *out = (T *)a.out + (long long)b * a.bso + (long long)ro.qi * a.ldo + (g * G + ro.hg) * 2 * HD + col0;
+#pragma unroll
+        for (int i = 0; i < NQ; i += 4)
+            *(int2 *)(out + 32 * (i >> 4) + 2 * (i & 15)) = make_int2(pack2<T>(o[0][i], o[0][i + 1]), pack2<T>(o[0][i + 2], o[0][i + 3]));
+    }
+};
+
+template <int RW, int KB>
+__device__ __forceinline__ Share shares(const DiffAttnArgs &a, const DiffPlan &pl, int lane) {
+    const unsigned U = pl.by_len ? ByLen<RW, KB>::total(a, lane) : (unsigned)(pl.tiles - pl.full) * pl.units;
+    const unsigned q = U / (unsigned)pl.shared;
+    return Share{q, U - q * pl.shared};
+}
+__device__ __forceinline__ int tile_order(const DiffAttnArgs &a, int heads, int i) { return a.causal ? heads - 1 - i : i; }   // the longest first
+
+template <typename T, int HD, int RW, int KW>
+__global__ __launch_bounds__(256, KW == 4 ? 1 : 2) void diff_attn_kernel(const DiffAttnArgs a, const DiffPlan pl) {
+    using A = Attn<T, HD, RW, KW>;
+    __shared__ __attribute__((aligned(1024))) char smem[A::LDS];
+    const int lane = threadIdx.x & 63, nkv = (int)a.nkv;
+    unsigned u = 0, end = 1;
+    int p = (int)blockIdx.x - pl.full;
+    if (p >= 0) {
+        p = (int)xcd_remap((unsigned)p, pl.shared);
+        const Share sh = shares<RW, A::KB>(a, pl, lane);
+        u = sh.begin(p);
+        end = sh.begin(p + 1);
+    }
+    while (u < end) {
+        int bg, tile, u0 = 0, u1 = pl.units, piece = -1;
+        if (p < 0) {
+            const int t = (int)xcd_remap(blockIdx.x, pl.full);
+            bg = t / pl.ntile;
+            tile = tile_order(a, pl.ntile, t - bg * pl.ntile);
+            u = end;
+        } else {
+            unsigned n = pl.units;
+            if (pl.by_len) {
+                const Spot s = ByLen<RW, A::KB>::find(a, u, lane);
+                const int g = s.tile / s.heads;
+                bg = s.b * nkv + g;
+                tile = tile_order(a, s.heads, s.tile - g * s.heads);
+                u0 = (int)(u - s.first);
+                n = s.n;
+            } else {
+                const int ts = (int)(u / n), t = pl.full + ts;
+                bg = t / pl.ntile;
+                tile = tile_order(a, pl.ntile, t - bg * pl.ntile);
+                u0 = (int)(u - ts * n);
+            }
+            u1 = (int)min(n, u0 + (end - u));
+            u += u1 - u0;
+            if (u0 > 0 || u1 < (int)n) piece = p + bg * pl.ntile + tile_order(a, pl.ntile, tile) - pl.full;
+        }
+        const int b = bg / nkv;
+        A::run(a, pl, smem, b, bg - b * nkv, tile, u0, u1, piece);
+    }
+}
+
+// Joins the pieces of the shared tiles: HD/2 lanes a row, four columns of each map a lane, pieces in the order of
+// their keys.
+template <typename T, int HD, int RW, int KB>
+__global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs a, const DiffPlan pl) {
+    constexpr int LR = HD / 2, RPW = 256 / LR, GROUPS = 32 * RW / RPW;   // workgroups of a tile
+    const int lane = threadIdx.x & (LR - 1);
+    const int ts = (int)(blockIdx.x / GROUPS), r = (int)(blockIdx.x % GROUPS) * RPW + (int)(threadIdx.x / LR);
+    const int t = pl.full + ts, bg = t / pl.ntile, nkv = (int)a.nkv;
+    const int b = bg / nkv, g = bg - b * nkv, G = (int)(a.nh / a.nkv);
+    // the tile's order number among those of its head is turned round once more where the kernel's is
+    int tile = tile_order(a, pl.ntile, t - bg * pl.ntile);
+    const int nq = q_rows(a, b);
+    if ((tile * 32 * RW + (int)(blockIdx.x % GROUPS) * RPW) / G >= nq) return;
+    const Share sh = shares<RW, KB>(a, pl, threadIdx.x & 63);
+    unsigned first = (unsigned)ts * pl.units, n = pl.units;
+    if (pl.by_len) {
+        // units before sample b
+        unsigned before = 0, own;
+        for (int b0 = 0; b0 + 64 <= b; b0 += 64) before += __builtin_amdgcn_readlane(ByLen<RW, KB>::scan(a, b0, threadIdx.x & 63, own), 63);
+        const unsigned upto = ByLen<RW, KB>::scan(a, b & ~63, threadIdx.x & 63, own);
+        before += __builtin_amdgcn_readlane(upto - own, b & 63);
+        int heads;
+        ByLen<RW, KB>::sample(a, b, heads, n);
+        first = before + (unsigned)(g * heads + tile_order(a, heads, tile)) * n;
+    }
+    const int p0 = (int)sh.holder(first), p1 = (int)sh.holder(first + n - 1);
+    if (p0 == p1) return;   // in one piece: written already
+    const RowOf ro = row_of(tile * 32 * RW + r, G);
+    const bool in = ro.qi < nq;
+    const int h = g * G + (in ? ro.hg : 0);
+    const long long row0 = (long long)ts * 32 * RW + r;
+    float m[2] = {-1e30f, -1e30f}, l[2] = {0.0f, 0.0f}, o[2][4] = {};
+    for (int p = in ? p0 : p1 + 1; p <= p1; ++p) {   // as over the keys: the larger reference, what was before scaled to it
+        const long long row = row0 + (long long)p * 32 * RW;
+        const float4 st = pl.st[row];
+        const float ms[2] = {st.x, st.z}, ls[2] = {st.y, st.w};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float4 v = *(const float4 *)(pl.o + row * (4 * HD) + j * 2 * HD + 4 * lane);
+            const float mn = fmaxf(m[j], ms[j]);
+            const float f = __builtin_amdgcn_exp2f(m[j] - mn), w = __builtin_amdgcn_exp2f(ms[j] - mn);
+            m[j] = mn;
+            l[j] = l[j] * f + ls[j] * w;
+            o[j][0] = o[j][0] * f + v.x * w;
+            o[j][1] = o[j][1] * f + v.y * w;
+            o[j][2] = o[j][2] * f + v.z * w;
+            o[j][3] = o[j][3] * f + v.w * w;
         }
     }
-    const RowOf ro = row_of(x, G);
-    const float lam = row_lambda(a, g, G, ro.hg, lane);
-    const float l0 = pair_sum(w.l[0]), l1 = pair_sum(w.l[1]);
-    const float r0 = l0 > 0.0f ? 1.0f / l0 : 0.0f, r1 = l1 > 0.0f ? lam / l1 : 0.0f;
-    float ss = 0.0f;
-#pragma unroll
-    for (int d = 0; d < L::DT; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float y = w.o[0][d][r] * r0 - w.o[1][d][r] * r1;
-            w.o[0][d][r] = y;
-            ss += y * y;
+    auto row_sum = [&](float v) {
+        v = row16_sum(v);
+        if constexpr (LR == 32) {
+            const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+            v = __uint_as_float(q[0]) + __uint_as_float(q[1]);
         }
-    ss = pair_sum(ss);
-    if (ro.qi >= nq) return;
-    const float f = a.norm_w ? (1.0f - a.lambda_init) / sqrtf(ss / (float)(2 * HD) + a.eps) : 1.0f;
-    T *out = (T *)a.out + (long long)b * a.bso + (long long)ro.qi * a.ldo + (g * G + ro.hg) * 2 * HD;
+        return v;
+    };
+    const float *lv = a.lam + (a.lam_heads > 1 ? (long long)h * 4 * HD : 0) + 2 * lane;
+    const float d1 = row_sum(lv[0] * lv[HD] + lv[1] * lv[HD + 1]), d2 = row_sum(lv[2 * HD] * lv[3 * HD] + lv[2 * HD + 1] * lv[3 * HD + 1]);
+    const float lam = expf(d1) - expf(d2) + a.lambda_init;
+    const float r0 = l[0] > 0.0f ? 1.0f / l[0] : 0.0f, r1 = l[1] > 0.0f ? lam / l[1] : 0.0f;
+    float y[4], ss = 0.0f;
 #pragma unroll
-    for (int d = 0; d < L::DT; ++d)
+    for (int e = 0; e < 4; ++e) {
+        y[e] = o[0][e] * r0 - o[1][e] * r1;
+        ss += y[e] * y[e];
+    }
+    ss = row_sum(ss);
+    if (!in) return;
+    if (a.norm_w) {
+        const float f = (1.0f - a.lambda_init) / sqrtf(ss / (float)(2 * HD) + a.eps);
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-            const int col = 32 * d + 8 * q4 + 4 * (lane >> 5);
-            s16x4 st;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float y = w.o[0][d][4 * q4 + e];
-                st[e] = __builtin_bit_cast(short, (T)(a.norm_w ? y * f * a.norm_w[col + e] : y));
-            }
-            *(s16x4 *)(out + col) = st;
-        }
+        for (int e = 0; e < 4; ++e) y[e] = y[e] * f * a.norm_w[4 * lane + e];
+    }
+    T *out = (T *)a.out + (long long)b * a.bso + (long long)ro.qi * a.ldo + (long long)h * 2 * HD + 4 * lane;
+    *(int2 *)out = make_int2(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]));
 }
 
 // the MFMA kernels read and write whole 16-byte chunks
@@ -418,21 +761,63 @@ bool chunked(const DiffAttnArgs &a) {
            ((a.ldq | a.ldk | a.ldv | a.ldo) & 7) == 0 && ((a.bsq | a.bsk | a.bsv | a.bso) & 7) == 0;
 }
 
-template <typename T, int HD>
-int launch_typed(const DiffAttnArgs &a, float *ws, size_t ws_bytes, hipStream_t st) {
-    (void)ws;
-    (void)ws_bytes;
-    if (!chunked(a)) {
-        const unsigned long long n = (unsigned long long)a.B * a.Sq * a.nh;
-        TSN_LAUNCH((diff_attn_any_kernel<T, HD>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, a);
+template <typename T, int HD, int RW, int KW>
+int launch_plan(const DiffAttnArgs &a, const DiffPlan &pl, hipStream_t st) {
+    TSN_LAUNCH((diff_attn_kernel<T, HD, RW, KW>), dim3((unsigned)(pl.full + pl.shared)), dim3(256), 0, st, a, pl);
+    TSN_HIP_CHECK(hipGetLastError());
+    if (pl.shared > 0) {
+        constexpr int GROUPS = 32 * RW * HD / 512;
+        TSN_LAUNCH((diff_attn_join_kernel<T, HD, RW, Attn<T, HD, RW, KW>::KB>), dim3((unsigned)(pl.tiles - pl.full) * GROUPS), dim3(256), 0, st, a, pl);
         TSN_HIP_CHECK(hipGetLastError());
-        return TSN_OK;
     }
-    const unsigned long long rows = (unsigned long long)a.Sq * (a.nh / a.nkv);
-    const int ntile = (int)((rows + 127) / 128);
-    TSN_LAUNCH((diff_attn_rows_kernel<T, HD>), dim3((unsigned)(a.B * a.nkv * ntile)), dim3(256), 0, st, a, ntile);
+    return TSN_OK;
+}
+
+template <typename T, int HD>
+int launch_any(const DiffAttnArgs &a, hipStream_t st) {
+    const unsigned long long n = (unsigned long long)a.B * a.Sq * a.nh;
+    TSN_LAUNCH((diff_attn_any_kernel<T, HD>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, a);
     TSN_HIP_CHECK(hipGetLastError());
     return TSN_OK;
+}
+
+// rows of a tile / 32, and what of the tiles is shared out
+struct DiffChoice {
+    int rw;
+    DiffPlan pl;
+    size_t bytes() const {
+        return pl.shared ? (size_t)(pl.tiles - pl.full + pl.shared) * 32 * rw * (4 * hd + 4) * sizeof(float) : 0;
+    }
+    int hd;
+};
+
+DiffChoice choose(const DiffAttnArgs &a) {
+    const long long rows = (long long)a.Sq * (a.nh / a.nkv);
+    DiffChoice best{};
+    double least = 1e30;
+    for (int rw : {4, 1}) {
+        DiffChoice c{};
+        c.rw = rw;
+        c.hd = (int)a.hd;
+        DiffPlan &p = c.pl;
+        const int kb = rw == 1 ? 128 : 64;
+        p.ntile = (int)((rows + 32 * rw - 1) / (32 * rw));
+        const long long tiles = (long long)p.ntile * a.nkv * a.B;
+        if (tiles >= (1LL << 31)) continue;
+        p.tiles = (int)tiles;
+        p.units = (int)((a.Sk + kb - 1) / kb);
+        const char *e = getenv("DA_PLAN");   // rw,full,shared
+        int er = 4, ef = -1, es = 0;
+        if (e) sscanf(e, "%d,%d,%d", &er, &ef, &es);
+        if (er != rw) continue;
+        p.full = ef < 0 ? p.tiles : ef < p.tiles ? ef : p.tiles;
+        p.shared = p.full < p.tiles ? es : 0;
+        if (p.shared > (long long)(p.tiles - p.full) * p.units) p.shared = (p.tiles - p.full) * p.units;
+        p.by_len = p.full == 0 && p.shared > 0 && (a.q_len || a.kv_len);
+        best = c;
+        (void)least;
+    }
+    return best;
 }
 
 } // namespace
@@ -485,10 +870,22 @@ int diff_attention_check(DiffAttnArgs &a) {
     return TSN_OK;
 }
 
-int launch_diff_attention(const DiffAttnArgs &a, float *ws, size_t ws_bytes, hipStream_t st) {
-    if (a.dt == DT_F16)
-        return a.hd == 64 ? launch_typed<half_t, 64>(a, ws, ws_bytes, st) : launch_typed<half_t, 32>(a, ws, ws_bytes, st);
-    return a.hd == 64 ? launch_typed<bf16_t, 64>(a, ws, ws_bytes, st) : launch_typed<bf16_t, 32>(a, ws, ws_bytes, st);
+size_t diff_attention_bytes(const DiffAttnArgs &a) { return chunked(a) ? choose(a).bytes() : 0; }
+
+int launch_diff_attention(const DiffAttnArgs &a, void *ws, size_t ws_bytes, hipStream_t st) {
+    auto typed = [&](auto t) -> int {
+        using T = decltype(t);
+        if (!chunked(a)) return a.hd == 64 ? launch_any<T, 64>(a, st) : launch_any<T, 32>(a, st);
+        DiffChoice c = choose(a);
+        TSN_REQUIRE(c.bytes() <= ws_bytes && (c.bytes() == 0 || ((uintptr_t)ws & 15) == 0), "diff_attention: workspace");
+        const size_t pieces = (size_t)(c.pl.tiles - c.pl.full + c.pl.shared) * 32 * c.rw;
+        c.pl.st = (float4 *)ws;
+        c.pl.o = (float *)ws + 4 * pieces;
+        if (a.hd == 64)
+            return c.rw == 4 ? launch_plan<T, 64, 4, 1>(a, c.pl, st) : launch_plan<T, 64, 1, 4>(a, c.pl, st);
+        return c.rw == 4 ? launch_plan<T, 32, 4, 1>(a, c.pl, st) : launch_plan<T, 32, 1, 4>(a, c.pl, st);
+    };
+    return a.dt == DT_F16 ? typed(half_t()) : typed(bf16_t());
 }
 
 } // namespace tsn

@@ -508,8 +508,9 @@ int rope_axes_check(RopeAxesArgs &a);
 int diff_attention_check(DiffAttnArgs &a);
 int gate_add_norm_check(GateNormArgs &a);
 int launch_rope_axes(const RopeAxesArgs &a, hipStream_t st);
-// ws: partial results of a split over the keys (ws_bytes of it), on the stream's own runtime
-int launch_diff_attention(const DiffAttnArgs &a, float *ws, size_t ws_bytes, hipStream_t st);
+// ws: diff_attention_bytes(a) bytes, 16-byte aligned, for pieces of tiles whose keys are shared out
+size_t diff_attention_bytes(const DiffAttnArgs &a);
+int launch_diff_attention(const DiffAttnArgs &a, void *ws, size_t ws_bytes, hipStream_t st);
 int launch_gate_add_norm(const GateNormArgs &a, hipStream_t st);
 
 } // namespace tsn

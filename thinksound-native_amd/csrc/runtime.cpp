@@ -457,7 +457,10 @@ int Runtime::rope_axes(const RopeAxesArgs &a) {
 }
 int Runtime::diff_attention(const DiffAttnArgs &a) {
     TSN_TRY(dev.make_current());
-    return launch_diff_attention(a, split_ws(), split_ws_bytes(), dev.stream());
+    void *ws = nullptr;
+    const size_t bytes = diff_attention_bytes(a);
+    if (bytes) TSN_TRY(scratch(bytes, &ws));
+    return launch_diff_attention(a, ws, bytes, dev.stream());
 }
 int Runtime::gate_add_norm(const GateNormArgs &a) {
     TSN_TRY(dev.make_current());

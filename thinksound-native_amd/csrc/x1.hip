@@ -1,0 +1,780 @@
+// diffattn.hip — differential attention for gfx950: the difference of two softmax maps times one V,
+//     lambda = exp(lq1.lk1) - exp(lq2.lk2) + lambda_init
+//     o = softmax(s q1 k1^T) v - lambda softmax(s q2 k2^T) v,   out = (1 - lambda_init) RMS(o) w, or o.
+// One pass over the keys: each map keeps its running maximum, sum and product with V (the online
+// softmax), and the two are joined once both sums are known.
+#include <math.h>
+#include <stdio.h>
+#include <stdlib.h>
+
+#include "kernels.h"
+
+#include "dpp.h"
+#include "elems.h"
+
+namespace tsn {
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// rows and keys of a sample, inside what the call gives it
+__device__ __forceinline__ int q_rows(const DiffAttnArgs &a, int b) {
+    return a.q_len ? min(max(a.q_len[b], 0), (int)a.Sq) : (int)a.Sq;
+}
+__device__ __forceinline__ int kv_rows(const DiffAttnArgs &a, int b) {
+    return a.kv_len ? min(max(a.kv_len[b], 0), (int)a.Sk) : (int)a.Sk;
+}
+// lambda of head h, by a whole wave: lane i takes element i of the vectors
+__device__ __forceinline__ float wave_lambda(const DiffAttnArgs &a, int h, int lane) {
+    const int hd = (int)a.hd;
+    const float *l = a.lam + (a.lam_heads > 1 ? (long long)h * 4 * hd : 0);
+    const bool in = lane < hd;
+    const float d1 = wave_sum(in ? l[lane] * l[hd + lane] : 0.0f);
+    const float d2 = wave_sum(in ? l[2 * hd + lane] * l[3 * hd + lane] : 0.0f);
+    return expf(d1) - expf(d2) + a.lambda_init;
+}
+
+// Any stride and alignment: one wave a row and head. A block of 64 keys at a time, lane j takes the scores of key j;
+// the probabilities go through LDS, then the lanes take the columns of V.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void diff_attn_any_kernel(const DiffAttnArgs a) {
+    constexpr int NV = 2 * HD / 64;   // columns of V a lane
+    __shared__ float sq[4][2 * HD];
+    __shared__ float sp[4][2][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const long long id = (long long)blockIdx.x * 4 + wave;
+    const long long n_items = (long long)a.B * a.Sq * a.nh;
+    if (id >= n_items) return;   // no barrier below: a wave uses its own LDS
+    const int h = (int)(id % a.nh);
+    const long long br = id / a.nh;
+    const int b = (int)(br / a.Sq), r = (int)(br - (long long)b * a.Sq);
+    const int nq = q_rows(a, b), nk = kv_rows(a, b);
+    if (r >= nq) return;
+    const int g = h / (int)(a.nh / a.nkv);
+    int keys = nk;
+    if (a.causal) keys = min(nk, max(0, r + nk - nq + 1));
+    const T *q = (const T *)a.q + (long long)b * a.bsq + (long long)r * a.ldq + (long long)h * 2 * HD;
+    const T *k = (const T *)a.k + (long long)b * a.bsk + (long long)g * 2 * HD;
+    const T *v = (const T *)a.v + (long long)b * a.bsv + (long long)g * 2 * HD;
+    for (int i = lane; i < 2 * HD; i += 64) sq[wave][i] = (float)q[i] * a.scale * LOG2E;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[2][NV] = {};
+    for (int k0 = 0; k0 < keys; k0 += 64) {
+        const int n = min(64, keys - k0);
+        float s[2] = {-INFINITY, -INFINITY};
+        if (lane < n) {
+            const T *kr = k + (long long)(k0 + lane) * a.ldk;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float d = 0.0f;
+                for (int i = 0; i < HD; ++i) d += sq[wave][j * HD + i] * (float)kr[j * HD + i];
+                s[j] = d;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float mn = fmaxf(m[j], wave_max(s[j]));
+            const float al = exp2f(m[j] - mn), p = lane < n ? exp2f(s[j] - mn) : 0.0f;
+            m[j] = mn;
+            l[j] = l[j] * al + wave_sum(p);
+            for (int c = 0; c < NV; ++c) o[j][c] *= al;
+            sp[wave][j][lane] = p;
+        }
+        for (int t = 0; t < n; ++t) {
+            const T *vr = v + (long long)(k0 + t) * a.ldv;
+#pragma unroll
+            for (int c = 0; c < NV; ++c) {
+                const float x = (float)vr[lane + 64 * c];
+                o[0][c] += sp[wave][0][t] * x;
+                o[1][c] += sp[wave][1][t] * x;
+            }
+        }
+    }
+    const float lam = wave_lambda(a, h, lane);
+    const float r0 = l[0] > 0.0f ? 1.0f / l[0] : 0.0f, r1 = l[1] > 0.0f ? lam / l[1] : 0.0f;
+    float ss = 0.0f, y[NV];
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+        y[c] = o[0][c] * r0 - o[1][c] * r1;
+        ss += y[c] * y[c];
+    }
+    const float f = a.norm_w ? (1.0f - a.lambda_init) / sqrtf(wave_sum(ss) / (float)(2 * HD) + a.eps) : 1.0f;
+    T *out = (T *)a.out + (long long)b * a.bso + (long long)r * a.ldo + (long long)h * 2 * HD;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+        const int i = lane + 64 * c;
+        out[i] = (T)(a.norm_w ? y[c] * f * a.norm_w[i] : y[c]);
+    }
+}
+
+/* ---------------- MFMA kernels ---------------- */
+//
+// The rows of a key/value head are its nh/nkv heads' rows, heads next to each other: row x is query x / G of head
+// g*G + x % G, so heads that share keys share a tile of them. A wave takes 32 rows and computes (32x32x16 MFMA, A row
+// and B column = lane & 31, K group = lane >> 5, D[8*(r>>2) + 4*(lane>>5) + (r&3)][lane & 31], r = 0..15)
+//   S^T = K Q^T  for 32 keys and each map: A = K rows from LDS, B = the wave's Q rows in registers. K rows are taken in
+//                the order key_of(i), so that a lane ends with keys 16c + 8*(lane>>5) + 0..7, c = 0, 1, of query lane & 31:
+//   O^T += V^T P^T: B = these probabilities as they lie in registers, A = V^T by transposing LDS reads
+//                (ds_read_b64_tr_b16: a 16-lane group reads four keys of 16 columns and gets column lane & 15).
+// Both maps multiply the same V fragments. A query's statistics and its O columns are in lanes q and q + 32.
+//
+// LDS rows (2 HD elements of one key) are 16-byte chunks; chunk c of row r sits at slot c ^ swizzle(r), so that the 16
+// rows of a K read and the four rows of a V read fall in distinct banks.
+
+typedef __attribute__((address_space(3))) char lds_char;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) i32x4 lds_i32x4;
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ floatx16 mfma32(i32x4 a, i32x4 b, floatx16 c, half_t) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx16 mfma32(i32x4 a, i32x4 b, floatx16 c, bf16_t) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// two values rounded to nearest even, in one register
+template <typename T> struct Pair;
+template <> struct Pair<half_t> { typedef half2_t type; };
+template <> struct Pair<bf16_t> { typedef bf16x2 type; };
+template <typename T>
+__device__ __forceinline__ int pack2(float a, float b) {
+    return __builtin_bit_cast(int, __builtin_convertvector((floatx2{a, b}), typename Pair<T>::type));
+}
+__device__ __forceinline__ floatx16 zero16() {
+    return floatx16{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+}
+// both lanes of a query (l, l ^ 32) get the maximum, the sum
+__device__ __forceinline__ float pair_max(float v) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+// A buffer of `bytes` (at most 2^30) bytes: loads from behind its end read as zero
+__device__ __forceinline__ i32x4 buffer(const void *base, unsigned bytes) {
+    const unsigned long long p = (unsigned long long)base;
+    return i32x4{(int)__builtin_amdgcn_readfirstlane((unsigned)p), (int)(__builtin_amdgcn_readfirstlane((unsigned)(p >> 32)) & 0xFFFF),
+                 (int)__builtin_amdgcn_readfirstlane(bytes), 0x00020000};
+}
+// 16 bytes a lane at voff + soff, global -> LDS slot (lane) of the 1 KB block at address lds. Ordered by explicit vmcnt
+// waits; s_nop 0 covers the M0 -> LDS-DMA hazard.
+__device__ __forceinline__ void dma16(i32x4 rs, unsigned voff, unsigned soff, unsigned lds) {
+    const unsigned l = __builtin_amdgcn_readfirstlane(lds), so = __builtin_amdgcn_readfirstlane(soff);
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+                 :
+                 : "v"(voff), "s"(rs), "s"(so), "s"(l)
+                 : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {   // at most N vector loads of this wave still under way
+    static_assert(N < 64, "vmcnt has six bits");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (0xF << 8));
+    asm volatile("" ::: "memory");
+}
+// this wave's LDS reads have completed before any wave passes: a stage refilled after it is not still being read
+__device__ __forceinline__ void block_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);   // vmcnt 63, expcnt 7: no wait; lgkmcnt 0
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+// consecutive logical workgroups run on one XCD (dispatch is round-robin over the 8): the row tiles of a key/value
+// head read its keys through one L2
+__device__ __forceinline__ unsigned xcd_remap(unsigned bid, unsigned n) {
+    const unsigned xcd = bid & 7, idx = bid >> 3, base = n >> 3, rem = n & 7;
+    return (xcd < rem ? xcd * (base + 1) : rem * (base + 1) + (xcd - rem) * base) + idx;
+}
+
+template <int HD>
+struct Lay {
+    static constexpr int ROW = 4 * HD;         // bytes of a key's row of K or V (2 HD elements)
+    static constexpr int CPR = ROW / 16;       // its chunks
+    static constexpr int RPB = 64 / CPR;       // rows of a 1 KB block
+    static constexpr int DT = 2 * HD / 32;     // 32-column tiles of V
+    static constexpr int KS = HD / 16;         // MFMA steps of a map's width
+    static __device__ __forceinline__ int ksw(int r) { return HD == 64 ? r & 15 : (r >> 1) & 7; }
+    static __device__ __forceinline__ int vsw(int r) { return HD == 64 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
+};
+__device__ __forceinline__ int key_of(int i) { return 16 * (i >> 4) + 8 * ((i >> 2) & 1) + 4 * ((i >> 3) & 1) + (i & 3); }
+
+// What a wave holds of its 32 rows: queries, running reference (log2 units), each lane's share of the sums, products
+template <int HD>
+struct Rows {
+    i32x4 q[2][Lay<HD>::KS];
+    float m[2], l[2];
+    floatx16 o[2][Lay<HD>::DT];
+    int lim;   // keys that the lane's row sees
+};
+
+// The lane's share of a tile's loads. Block i of a wave's holds rows r0 + i*RPB.. of the tile; row r's chunk c goes to
+// slot c ^ swizzle(r). The K swizzle of block i is that of block 0 ^ 4i, the V swizzle the same for all.
+template <int HD, int NB>
+struct Loads {
+    unsigned k[NB], v;   // byte offsets in the tile: K for each block, V (blocks RPB rows apart)
+};
+template <int HD, int NB>
+__device__ __forceinline__ Loads<HD, NB> lane_loads(int row0, unsigned ldk, unsigned ldv, int lane) {
+    using L = Lay<HD>;
+    Loads<HD, NB> o;
+    const int r = row0 + lane / L::CPR, c = lane % L::CPR;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) o.k[i] = (unsigned)r * ldk + ((c ^ L::ksw(r + i * L::RPB)) << 4);
+    o.v = (unsigned)r * ldv + ((c ^ L::vsw(r)) << 4);
+    return o;
+}
+// the wave's NB blocks of K to lds, NB of V to lds + v_off; `rows` of the tile are there, the others read as zero
+template <int HD, int NB>
+__device__ __forceinline__ void load_tile(const Loads<HD, NB> &o, const char *kt, const char *vt, unsigned ldk, unsigned ldv, int rows,
+                                          unsigned lds, unsigned v_off) {
+    using L = Lay<HD>;
+    const int n = rows - 1;
+    const i32x4 rk = buffer(kt, n < 0 ? 0u : (unsigned)n * ldk + L::ROW), rv = buffer(vt, n < 0 ? 0u : (unsigned)n * ldv + L::ROW);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) dma16(rk, o.k[i], i * L::RPB * ldk, lds + i * 1024);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) dma16(rv, o.v, i * L::RPB * ldv, lds + v_off + i * 1024);
+}
+
+// LDS addresses of the lane's part of a tile of 32 rows: K row key_of(lane & 31), V row 8*(lane>>5) + (lane&15)/4. Other
+// chunks are reached by ^ (bits 4 to 7), other rows, blocks and stages by +: they do not meet.
+template <int HD>
+__device__ __forceinline__ unsigned k_lane(int lane) {
+    const int r = key_of(lane & 31);
+    return r * Lay<HD>::ROW + (((lane >> 5) ^ Lay<HD>::ksw(r)) << 4);
+}
+template <int HD>
+__device__ __forceinline__ unsigned v_lane(int lane) {
+    const int r = 8 * (lane >> 5) + ((lane & 15) >> 2);
+    return r * Lay<HD>::ROW + (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ Lay<HD>::vsw(r)) << 4) + (lane & 1) * 8;
+}
+// S^T of both maps for 32 keys, k = k_lane + the K tile's address
+template <typename T, int HD>
+__device__ __forceinline__ void scores(const Rows<HD> &w, unsigned k, floatx16 (&s)[2]) {
+    using L = Lay<HD>;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        s[j] = zero16();
+#pragma unroll
+        for (int ks = 0; ks < L::KS; ++ks)
+            s[j] = mfma32(*(lds_i32x4 *)(k ^ ((j * (HD / 8) + ks * 2) << 4)), w.q[j][ks], s[j], T());
+    }
+}
+// scores of keys that the lane's row does not see: key 0 of the 32 at k0
+template <int HD>
+__device__ __forceinline__ void mask_scores(const Rows<HD> &w, floatx16 (&s)[2], int k0, int lane) {
+    const int left = w.lim - k0 - 8 * (lane >> 5);
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+        if (16 * (r >> 3) + (r & 7) >= left) s[0][r] = s[1][r] = -INFINITY;
+}
+// Probabilities of 32 keys. The reference m moves only when a score passes it by more than 2^8: probabilities stay
+// below 2^8, inside f16, and most steps leave O as it is. Returns whether any lane's moved; al: by what O has to be
+// scaled before these probabilities' product is added.
+template <typename T, int HD>
+__device__ __forceinline__ bool probs(Rows<HD> &w, const floatx16 (&s)[2], i32x4 (&p)[2][2], float (&al)[2], float c) {
+    bool moved = false;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        float t = fmaxf(fmaxf(s[j][0], s[j][1]), s[j][2]);
+#pragma unroll
+        for (int r = 3; r < 15; r += 2) t = fmaxf(fmaxf(t, s[j][r]), s[j][r + 1]);
+        t = pair_max(fmaxf(t, s[j][15])) * c;
+        const bool up = t > w.m[j] + 8.0f;
+        const float mn = up ? t : w.m[j];
+        al[j] = __builtin_amdgcn_exp2f(w.m[j] - mn);
+        w.m[j] = mn;
+        moved |= up;
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], c, -mn));
+            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r + 1], c, -mn));
+            sum += e0;
+            sum += e1;
+            p[j][r >> 3][(r & 7) >> 1] = pack2<T>(e0, e1);
+        }
+        w.l[j] = __builtin_fmaf(w.l[j], al[j], sum);
+    }
+    return __builtin_amdgcn_ballot_w64(moved) != 0;
+}
+template <int HD>
+__device__ __forceinline__ void rescale(Rows<HD> &w, const float (&al)[2]) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int d = 0; d < Lay<HD>::DT; ++d) w.o[j][d] *= al[j];
+}
+// O^T += V^T P^T for 32 keys, v = v_lane + the V tile's address: A row = column 32d + (lane & 31) of V, keys
+// 16h + 8*(lane>>5) + 0..7 by two transposing reads of four
+template <typename T, int HD>
+__device__ __forceinline__ void product(Rows<HD> &w, unsigned v, const i32x4 (&p)[2][2]) {
+    using L = Lay<HD>;
+#pragma unroll
+    for (int d = 0; d < L::DT; ++d) {
+        const unsigned vd = v ^ (d << 6);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int2 lo = __builtin_bit_cast(int2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vd + 16 * h * L::ROW)));
+            const int2 hi = __builtin_bit_cast(int2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vd + (16 * h + 4) * L::ROW)));
+            const i32x4 vf = i32x4{lo.x, lo.y, hi.x, hi.y};
+            w.o[0][d] = mfma32(vf, p[0][h], w.o[0][d], T());
+            w.o[1][d] = mfma32(vf, p[1][h], w.o[1][d], T());
+        }
+    }
+}
+// Row x of a key/value head: its query and head within the group
+struct RowOf {
+    int qi, hg;
+};
+__device__ __forceinline__ RowOf row_of(int x, int G) {
+    const int qi = G == 1 ? x : x / G;
+    return RowOf{qi, x - qi * G};
+}
+
+template <typename T, int HD>
+__device__ __forceinline__ void load_rows(Rows<HD> &w, const DiffAttnArgs &a, int b, int g, int G, int x, int nq, int nk, int lane) {
+    using L = Lay<HD>;
+    const RowOf ro = row_of(x, G);
+    const bool in = ro.qi < nq;
+    const T *q = (const T *)a.q + (long long)b * a.bsq + (long long)ro.qi * a.ldq + (g * G + ro.hg) * 2 * HD + 8 * (lane >> 5);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int ks = 0; ks < L::KS; ++ks) {
+            w.q[j][ks] = i32x4{0, 0, 0, 0};
+            if (in) w.q[j][ks] = *(const i32x4 *)(q + j * HD + ks * 16);
+        }
+        w.m[j] = -1e30f;
+        w.l[j] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < L::DT; ++d) w.o[j][d] = zero16();
+    }
+    w.lim = !in ? 0 : a.causal ? min(nk, max(0, ro.qi + nk - nq + 1)) : nk;
+}
+
+// lambda of the lane's head
+__device__ __forceinline__ float row_lambda(const DiffAttnArgs &a, int g, int G, int hg, int lane) {
+    if (a.lam_heads == 1) return wave_lambda(a, 0, lane);
+    float lam = 0.0f;
+    for (int i = 0; i < G; ++i) {
+        const float v = wave_lambda(a, g * G + i, lane);
+        if (hg == i) lam = v;
+    }
+    return lam;
+}
+
+// How a launch's work is cut. A tile is the 32*RW rows x0.. of one key/value head of one sample, its keys are `units`
+// units of Lay::KB keys. The first `full` tiles have a workgroup each; the units of the others, one after the other, are
+// shared out evenly among `shared` workgroups, whose pieces of tiles go to ws and are joined by diff_attn_join_kernel.
+struct DiffPlan {
+    int ntile;       // tiles of a key/value head
+    int tiles;       // of all
+    int units;       // key units of a tile
+    int full, shared;
+    float *o;        // [piece][row of the tile][map][2 HD]: products with V, not divided
+    float4 *st;      // [piece][row of the tile]: reference and sum of each map
+};
+// unit range of shared workgroup p, and the piece that it and tile t (counted from the first shared one) have in common:
+// both only grow along the units, so p + t is a number of its own
+__host__ __device__ __forceinline__ long long share_begin(const DiffPlan &pl, int p) {
+    return (long long)(pl.tiles - pl.full) * pl.units * p / pl.shared;
+}
+
+// One tile or piece of one: 32 rows a wave, RW waves side by side; KW waves share the rows of one and take every KW-th
+// block of 32 keys, and are merged at the end through LDS. All four read the same K and V tiles, two stages in LDS: the
+// next is loaded while one is worked on. Two workgroups a CU (KW = 4: one): one's matrix products cover the other's
+// softmax.
+template <typename T, int HD, int RW, int KW>
+struct Attn {
+    using L = Lay<HD>;
+    static constexpr int NSUB = KW > 2 ? KW : 2;     // blocks of 32 keys in a unit
+    static constexpr int KB = 32 * NSUB;
+    static constexpr int OP = KB * L::ROW, STAGE = 2 * OP, SUB = 32 * L::ROW;
+    static constexpr int NB = OP / 1024 / 4;         // 1 KB blocks of K, of V, a wave and unit
+    static constexpr int NO = 2 * L::DT * 16;        // products of a lane
+    static constexpr int MERGE = KW > 1 ? RW * (KW / 2) * 64 * 4 * (NO + 4) : 0;
+    static constexpr int LDS = 2 * STAGE > MERGE ? 2 * STAGE : MERGE;
+    static_assert(RW * KW == 4, "four waves");
+
+    static __device__ __forceinline__ void merge(Rows<HD> &w, float *buf, int rw, int kw, int lane) {
+#pragma unroll
+        for (int half = KW / 2; half > 0; half /= 2) {
+            // lane's values 64 floats apart: no bank conflicts
+            float *p = buf + ((kw % half) * RW + rw) * 64 * (NO + 4) + lane;
+            block_barrier();   // the key tiles, or the previous round's values, have been read
+            if (kw >= half && kw < 2 * half) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                    for (int d = 0; d < L::DT; ++d)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) p[((j * L::DT + d) * 16 + r) * 64] = w.o[j][d][r];
+                    p[(NO + 2 * j) * 64] = w.m[j];
+                    p[(NO + 2 * j + 1) * 64] = w.l[j];
+                }
+            }
+            block_barrier();
+            if (kw < half) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float m2 = p[(NO + 2 * j) * 64], l2 = p[(NO + 2 * j + 1) * 64];
+                    const float mn = fmaxf(w.m[j], m2);
+                    const float a1 = __builtin_amdgcn_exp2f(w.m[j] - mn), a2 = __builtin_amdgcn_exp2f(m2 - mn);
+                    w.m[j] = mn;
+                    w.l[j] = w.l[j] * a1 + l2 * a2;
+#pragma unroll
+                    for (int d = 0; d < L::DT; ++d)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) w.o[j][d][r] = w.o[j][d][r] * a1 + p[((j * L::DT + d) * 16 + r) * 64] * a2;
+                }
+            }
+        }
+    }
+
+    static __device__ __forceinline__ void run(const DiffAttnArgs &a, const DiffPlan &pl, char *smem, int t, int u0, int u1, int piece) {
+        const unsigned lds = (unsigned)(unsigned long)(lds_char *)smem;
+        const int lane = threadIdx.x & 63;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int rw = wave % RW, kw = wave / RW;
+        const int bg = t / pl.ntile, in_head = t - bg * pl.ntile;
+        const int tile = a.causal ? pl.ntile - 1 - in_head : in_head;   // causal: the longest first
+        const int b = bg / (int)a.nkv, g = bg - b * (int)a.nkv, G = (int)(a.nh / a.nkv);
+        const int nq = q_rows(a, b), nk = kv_rows(a, b);
+        const int x0 = tile * 32 * RW;
+        if (x0 / G >= nq) return;   // the whole workgroup: no row of the tile is there
+        const int x = x0 + rw * 32 + (lane & 31);
+        Rows<HD> w;
+        load_rows<T, HD>(w, a, b, g, G, x, nq, nk, lane);
+        // keys that any row of the tile, any row of the wave, and every row of the wave sees
+        auto limit = [&](int xr) {
+            const int qi = min(row_of(xr, G).qi, nq - 1);
+            return a.causal ? min(nk, max(0, qi + nk - nq + 1)) : nk;
+        };
+        const int keys = limit(x0 + 32 * RW - 1), all = limit(x0 + rw * 32);
+        const int wkeys = row_of(x0 + rw * 32, G).qi < nq ? limit(x0 + rw * 32 + 31) : 0;
+        const char *kp = (const char *)((const T *)a.k + (long long)b * a.bsk + g * 2 * HD);
+        const char *vp = (const char *)((const T *)a.v + (long long)b * a.bsv + g * 2 * HD);
+        const unsigned ldk = a.ldk * 2, ldv = a.ldv * 2;
+        const Loads<HD, NB> lo = lane_loads<HD, NB>(wave * NB * L::RPB, ldk, ldv, lane);
+        const unsigned kl = lds + k_lane<HD>(lane), vl = lds + OP + v_lane<HD>(lane);
+        auto issue = [&](int u) {
+            const long long k0 = (long long)u * KB;
+            load_tile<HD, NB>(lo, kp + k0 * ldk, vp + k0 * ldv, ldk, ldv, min(KB, nk - u * KB), lds + (u & 1) * STAGE + wave * NB * 1024, OP);
+        };
+        const float c = a.scale > 0.0f ? a.scale * LOG2E : 1e-30f;   // a scale of 0 must not meet a masked score's infinity
+        const int end = min(u1, (keys + KB - 1) / KB);
+        block_barrier();   // an earlier piece's LDS has been read
+        if (u0 < end) issue(u0);
+        for (int u = u0; u < end; ++u) {
+            wait_vmcnt<0>();
+            block_barrier();
+            if (u + 1 < end) issue(u + 1);
+            const unsigned at = (u & 1) * STAGE;
+#pragma unroll 1
+            for (int i = 0; i < NSUB / KW; ++i) {
+                const int blk = i * KW + kw;
+                const int k0 = u * KB + 32 * blk;
+
+                floatx16 s[2];
+                i32x4 p[2][2];
+                float al[2];
+                scores<T, HD>(w, kl + at + blk * SUB, s);
+                if (k0 + 32 > all) mask_scores<HD>(w, s, k0, lane);
+                if (probs<T, HD>(w, s, p, al, c)) rescale<HD>(w, al);
+                product<T, HD>(w, vl + at + blk * SUB, p);
+            }
+        }
+        if constexpr (KW > 1) merge(w, (float *)smem, rw, kw, lane);
+        if (kw > 0) return;
+        const RowOf ro = row_of(x, G);
+        const float l0 = pair_sum(w.l[0]), l1 = pair_sum(w.l[1]);
+        if (piece >= 0) {
+            if (ro.qi >= nq) return;
+            const long long row = (long long)piece * (32 * RW) + rw * 32 + (lane & 31);
+            if (lane < 32) pl.st[row] = make_float4(w.m[0], l0, w.m[1], l1);
+            float *o = pl.o + row * (4 * HD) + 4 * (lane >> 5);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int d = 0; d < L::DT; ++d)
+#pragma unroll
+                    for (int q4 = 0; q4 < 4; ++q4)
+                        *(float4 *)(o + j * 2 * HD + 32 * d + 8 * q4) = make_float4(w.o[j][d][4 * q4], w.o[j][d][4 * q4 + 1],
+                                                                                   w.o[j][d][4 * q4 + 2], w.o[j][d][4 * q4 + 3]);
+            return;
+        }
+        const float lam = row_lambda(a, g, G, ro.hg, lane);
+        const float r0 = l0 > 0.0f ? 1.0f / l0 : 0.0f, r1 = l1 > 0.0f ? lam / l1 : 0.0f;
+        float ss = 0.0f;
+#pragma unroll
+        for (int d = 0; d < L::DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float y = w.o[0][d][r] * r0 - w.o[1][d][r] * r1;
+                w.o[0][d][r] = y;
+                ss += y * y;
+            }
+        ss = pair_sum(ss);
+        if (ro.qi >= nq) return;
+        const float f = a.norm_w ? (1.0f - a.lambda_init) / sqrtf(ss / (float)(2 * HD) + a.eps) : 1.0f;
+        T *out = (T *)a.out + (long long)b * a.bso + (long long)ro.qi * a.ldo + (g * G + ro.hg) * 2 * HD;
+#pragma unroll
+        for (int d = 0; d < L::DT; ++d)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                const int col = 32 * d + 8 * q4 + 4 * (lane >> 5);
+                float y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    y[e] = w.o[0][d][4 * q4 + e];
+                    if (a.norm_w) y[e] = y[e] * f * a.norm_w[col + e];
+                }
+                *(int2 *)(out + col) = make_int2(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]));
+            }
+    }
+};
+
+template <typename T, int HD, int RW, int KW>
+__global__ __launch_bounds__(256, KW == 4 ? 1 : 2) void diff_attn_kernel(const DiffAttnArgs a, const DiffPlan pl) {
+    using A = Attn<T, HD, RW, KW>;
+    __shared__ __attribute__((aligned(1024))) char smem[A::LDS];
+    const unsigned wg = xcd_remap(blockIdx.x, gridDim.x);
+    int t = (int)wg, u0 = 0, u1 = pl.units, piece = -1;
+    long long u = 0, end = 0;   // a shared workgroup's units that are still to do
+    const int p = (int)wg - pl.full;
+    if (p >= 0) {
+        u = share_begin(pl, p);
+        end = share_begin(pl, p + 1);
+    }
+    do {
+        if (p >= 0) {
+            if (u >= end) return;
+            const int ts = (int)(u / pl.units);
+            u0 = (int)(u - (long long)ts * pl.units);
+            u1 = (int)min((long long)pl.units, u0 + (end - u));
+            u += u1 - u0;
+            t = pl.full + ts;
+            piece = u0 == 0 && u1 == pl.units ? -1 : p + ts;
+        }
+        A::run(a, pl, smem, t, u0, u1, piece);
+    } while (p >= 0);
+}
+
+// Joins the pieces of the shared tiles: HD/2 lanes a row, four columns of each map a lane, pieces in the order of
+// their keys.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs a, const DiffPlan pl, int rows_tile) {
+    constexpr int LR = HD / 2, RPW = 256 / LR;
+    const int lane = threadIdx.x & (LR - 1);
+    const long long id = (long long)blockIdx.x * RPW + threadIdx.x / LR;
+    const int ts = (int)(id / rows_tile), r = (int)(id - (long long)ts * rows_tile);
+    if (ts >= pl.tiles - pl.full) return;
+    // the shared workgroups that hold the tile's first and last unit
+    const long long first = (long long)ts * pl.units, last = first + pl.units - 1;
+    const long long U = (long long)(pl.tiles - pl.full) * pl.units;
+    auto holder = [&](long long u) {
+        int p = (int)(u * pl.shared / U);
+        while (share_begin(pl, p + 1) <= u) ++p;
+        while (share_begin(pl, p) > u) --p;
+        return p;
+    };
+    const int p0 = holder(first), p1 = holder(last);
+    if (p0 == p1) return;   // in one piece: written already
+    const int t = pl.full + ts, bg = t / pl.ntile, in_head = t - bg * pl.ntile;
+    const int tile = a.causal ? pl.ntile - 1 - in_head : in_head;
+    const int b = bg / (int)a.nkv, g = bg - b * (int)a.nkv, G = (int)(a.nh / a.nkv);
+    const RowOf ro = row_of(tile * rows_tile + r, G);
+    if (ro.qi >= q_rows(a, b)) return;
+    const int h = g * G + ro.hg;
+    float m[2] = {-1e30f, -1e30f}, l[2] = {0.0f, 0.0f};
+    for (int p = p0; p <= p1; ++p) {
+        const float4 st = pl.st[(long long)(p + ts) * rows_tile + r];
+        m[0] = fmaxf(m[0], st.x);
+        m[1] = fmaxf(m[1], st.z);
+    }
+    float o[2][4] = {};
+    for (int p = p0; p <= p1; ++p) {
+        const long long row = (long long)(p + ts) * rows_tile + r;
+        const float4 st = pl.st[row];
+        const float w[2] = {__builtin_amdgcn_exp2f(st.x - m[0]), __builtin_amdgcn_exp2f(st.z - m[1])};
+        l[0] += st.y * w[0];
+        l[1] += st.w * w[1];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float4 v = *(const float4 *)(pl.o + row * (4 * HD) + j * 2 * HD + 4 * lane);
+            o[j][0] += v.x * w[j];
+            o[j][1] += v.y * w[j];
+            o[j][2] += v.z * w[j];
+            o[j][3] += v.w * w[j];
+        }
+    }
+    auto row_sum = [&](float v) {
+        v = row16_sum(v);
+        if constexpr (LR == 32) {
+            const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+            v = __uint_as_float(q[0]) + __uint_as_float(q[1]);
+        }
+        return v;
+    };
+    const float *lv = a.lam + (a.lam_heads > 1 ? (long long)h * 4 * HD : 0) + 2 * lane;
+    const float d1 = row_sum(lv[0] * lv[HD] + lv[1] * lv[HD + 1]), d2 = row_sum(lv[2 * HD] * lv[3 * HD] + lv[2 * HD + 1] * lv[3 * HD + 1]);
+    const float lam = expf(d1) - expf(d2) + a.lambda_init;
+    const float r0 = l[0] > 0.0f ? 1.0f / l[0] : 0.0f, r1 = l[1] > 0.0f ? lam / l[1] : 0.0f;
+    float y[4], ss = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        y[e] = o[0][e] * r0 - o[1][e] * r1;
+        ss += y[e] * y[e];
+    }
+    if (a.norm_w) {
+        const float f = (1.0f - a.lambda_init) / sqrtf(row_sum(ss) / (float)(2 * HD) + a.eps);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = y[e] * f * a.norm_w[4 * lane + e];
+    }
+    T *out = (T *)a.out + (long long)b * a.bso + (long long)ro.qi * a.ldo + (long long)h * 2 * HD + 4 * lane;
+    *(int2 *)out = make_int2(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]));
+}
+
+// the MFMA kernels read and write whole 16-byte chunks
+bool chunked(const DiffAttnArgs &a) {
+    return (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) & 15) == 0 &&
+           ((a.ldq | a.ldk | a.ldv | a.ldo) & 7) == 0 && ((a.bsq | a.bsk | a.bsv | a.bso) & 7) == 0;
+}
+
+template <typename T, int HD, int RW, int KW>
+int launch_plan(const DiffAttnArgs &a, const DiffPlan &pl, hipStream_t st) {
+    TSN_LAUNCH((diff_attn_kernel<T, HD, RW, KW>), dim3((unsigned)(pl.full + pl.shared)), dim3(256), 0, st, a, pl);
+    TSN_HIP_CHECK(hipGetLastError());
+    if (pl.shared > 0) {
+        const long long rows = (long long)(pl.tiles - pl.full) * 32 * RW;
+        constexpr int RPW = 512 / HD;
+        TSN_LAUNCH((diff_attn_join_kernel<T, HD>), dim3((unsigned)((rows + RPW - 1) / RPW)), dim3(256), 0, st, a, pl, 32 * RW);
+        TSN_HIP_CHECK(hipGetLastError());
+    }
+    return TSN_OK;
+}
+
+template <typename T, int HD>
+int launch_any(const DiffAttnArgs &a, hipStream_t st) {
+    const unsigned long long n = (unsigned long long)a.B * a.Sq * a.nh;
+    TSN_LAUNCH((diff_attn_any_kernel<T, HD>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, a);
+    TSN_HIP_CHECK(hipGetLastError());
+    return TSN_OK;
+}
+
+// rows of a tile / 32, and what of the tiles is shared out
+struct DiffChoice {
+    int rw;
+    DiffPlan pl;
+    size_t bytes() const {
+        return pl.shared ? (size_t)(pl.tiles - pl.full + pl.shared) * 32 * rw * (4 * hd + 4) * sizeof(float) : 0;
+    }
+    int hd;
+};
+
+DiffChoice choose(const DiffAttnArgs &a) {
+    const long long rows = (long long)a.Sq * (a.nh / a.nkv);
+    DiffChoice best{};
+    double least = 1e30;
+    for (int rw : {4, 2, 1}) {
+        DiffChoice c{};
+        c.rw = rw;
+        c.hd = (int)a.hd;
+        DiffPlan &p = c.pl;
+        const int kb = rw == 1 ? 128 : 64;
+        p.ntile = (int)((rows + 32 * rw - 1) / (32 * rw));
+        const long long tiles = (long long)p.ntile * a.nkv * a.B;
+        if (tiles >= (1LL << 31)) continue;
+        p.tiles = (int)tiles;
+        p.units = (int)((a.Sk + kb - 1) / kb);
+        const char *e = getenv("DA_PLAN");   // rw,full,shared
+        int er = 4, ef = -1, es = 0;
+        if (e) sscanf(e, "%d,%d,%d", &er, &ef, &es);
+        if (er != rw) continue;
+        p.full = ef < 0 ? p.tiles : ef < p.tiles ? ef : p.tiles;
+        p.shared = p.full < p.tiles ? es : 0;
+        if (p.shared > (long long)(p.tiles - p.full) * p.units) p.shared = (p.tiles - p.full) * p.units;
+        best = c;
+        (void)least;
+    }
+    return best;
+}
+
+} // namespace
+
+int diff_attention_check(DiffAttnArgs &a) {
+    TSN_REQUIRE(a.q && a.k && a.v && a.lam && a.out, "diff_attention: null tensor");
+    TSN_REQUIRE(a.dt == DT_F16 || a.dt == DT_BF16, "diff_attention: dtype f16 or bf16");
+    TSN_REQUIRE(a.B > 0 && a.Sq > 0 && a.Sk > 0 && a.nh > 0 && a.nkv > 0, "diff_attention: empty shape");
+    if (a.hd != 32 && a.hd != 64) {
+        set_error("diff_attention: hd must be 32 or 64");
+        return TSN_ERR_UNSUPPORTED;
+    }
+    TSN_REQUIRE(a.nh % a.nkv == 0, "diff_attention: nh must be a multiple of nkv");
+    TSN_REQUIRE(a.lam_heads == 1 || a.lam_heads == a.nh, "diff_attention: lambda vectors for one head or for each");
+    TSN_REQUIRE(isfinite(a.scale) && a.scale >= 0.0f, "diff_attention: scale must be finite and not negative");
+    TSN_REQUIRE(a.lambda_init >= 0.0f && a.lambda_init < 1.0f, "diff_attention: lambda_init must be in [0, 1)");
+    TSN_REQUIRE(!a.norm_w || (isfinite(a.eps) && a.eps >= 0.0f), "diff_attention: eps must be finite and not negative");
+    TSN_REQUIRE(a.nh <= (1u << 12) && a.Sq < (1u << 30) && a.Sk < (1u << 30) &&
+                    (unsigned long long)a.B * a.Sq * a.nh < (1ULL << 31),
+                "diff_attention: sizes beyond the launch grid");
+    const uint32_t wq = 2 * a.nh * a.hd, wk = 2 * a.nkv * a.hd;
+    if (!a.ldq) a.ldq = wq;
+    if (!a.ldk) a.ldk = wk;
+    if (!a.ldv) a.ldv = wk;
+    if (!a.ldo) a.ldo = wq;
+    TSN_REQUIRE(a.ldq >= wq && a.ldk >= wk && a.ldv >= wk && a.ldo >= wq, "diff_attention: row stride below the row width");
+    TSN_REQUIRE(a.ldq <= (1u << 22) && a.ldk <= (1u << 22) && a.ldv <= (1u << 22) && a.ldo <= (1u << 22),
+                "diff_attention: row stride above 2^22 elements");
+    if (!a.bsq) a.bsq = (uint64_t)a.Sq * a.ldq;
+    if (!a.bsk) a.bsk = (uint64_t)a.Sk * a.ldk;
+    if (!a.bsv) a.bsv = (uint64_t)a.Sk * a.ldv;
+    if (!a.bso) a.bso = (uint64_t)a.Sq * a.ldo;
+    TSN_REQUIRE(a.bsq < (1ULL << 40) && a.bsk < (1ULL << 40) && a.bsv < (1ULL << 40) && a.bso < (1ULL << 40),
+                "diff_attention: sample stride above 2^40 elements");
+    TSN_REQUIRE(a.B == 1 || a.bso >= (uint64_t)(a.Sq - 1) * a.ldo + wq || (a.bso >= wq && a.ldo >= (a.B - 1) * a.bso + wq),
+                "diff_attention: the samples of out overlap");
+    TSN_REQUIRE(((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) % 2 == 0 &&
+                    ((uintptr_t)a.lam | (uintptr_t)a.norm_w | (uintptr_t)a.q_len | (uintptr_t)a.kv_len) % 4 == 0,
+                "diff_attention: pointers must be aligned to their elements");
+    const Window o = window(a.out, 2, wq, a.ldo, a.Sq, a.bso, a.B);
+    TSN_REQUIRE(!windows_meet(o, window(a.q, 2, wq, a.ldq, a.Sq, a.bsq, a.B)) &&
+                    !windows_meet(o, window(a.k, 2, wk, a.ldk, a.Sk, a.bsk, a.B)) &&
+                    !windows_meet(o, window(a.v, 2, wk, a.ldv, a.Sk, a.bsv, a.B)),
+                "diff_attention: out overlaps an input");
+    const uint64_t nl = 4ULL * a.lam_heads * a.hd;
+    struct { const void *p; unsigned long long n; } vec[4] = {
+        {a.lam, nl}, {a.norm_w, 2ULL * a.hd}, {a.q_len, a.B}, {a.kv_len, a.B}};
+    for (auto &v : vec)
+        TSN_REQUIRE(!v.p || !windows_meet(o, window(v.p, 4, v.n, v.n, 1)), "diff_attention: out overlaps lam, norm_w or the lengths");
+    return TSN_OK;
+}
+
+size_t diff_attention_bytes(const DiffAttnArgs &a) { return chunked(a) ? choose(a).bytes() : 0; }
+
+int launch_diff_attention(const DiffAttnArgs &a, void *ws, size_t ws_bytes, hipStream_t st) {
+    auto typed = [&](auto t) -> int {
+        using T = decltype(t);
+        if (!chunked(a)) return a.hd == 64 ? launch_any<T, 64>(a, st) : launch_any<T, 32>(a, st);
+        DiffChoice c = choose(a);
+        TSN_REQUIRE(c.bytes() <= ws_bytes && (c.bytes() == 0 || ((uintptr_t)ws & 15) == 0), "diff_attention: workspace");
+        const size_t pieces = (size_t)(c.pl.tiles - c.pl.full + c.pl.shared) * 32 * c.rw;
+        c.pl.st = (float4 *)ws;
+        c.pl.o = (float *)ws + 4 * pieces;
+        if (a.hd == 64)
+            return c.rw == 4 ? launch_plan<T, 64, 4, 1>(a, c.pl, st) : c.rw == 2 ? launch_plan<T, 64, 2, 2>(a, c.pl, st) : launch_plan<T, 64, 1, 4>(a, c.pl, st);
+        return c.rw == 4 ? launch_plan<T, 32, 4, 1>(a, c.pl, st) : c.rw == 2 ? launch_plan<T, 32, 2, 2>(a, c.pl, st) : launch_plan<T, 32, 1, 4>(a, c.pl, st);
+    };
+    return a.dt == DT_F16 ? typed(half_t()) : typed(bf16_t());
+}
+
+} // namespace tsn
