@@ -23,7 +23,10 @@ COMMON = ["-std=c++17", "-O3", "-fPIC", "-Wall", "-Wno-unused-function",
 
 # attention.hip produces no NaN (every key block holds a valid key, masked scores are -inf): with
 # NaNs ruled out the compiler drops the quieting max before each max of the softmax
-EXTRA = {"attention.hip": ["-fno-honor-nans", "-mno-amdgpu-ieee"]}
+EXTRA = {"attention.hip": ["-fno-honor-nans", "-mno-amdgpu-ieee"],
+         # products stay in VGPRs, where the softmax reads and rescales them (the kernel for few rows has a SIMD's
+         # whole register file a wave and would get AGPRs, and two moves for every value)
+         "diffattn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _compile(src):

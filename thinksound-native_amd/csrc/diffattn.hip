@@ -260,13 +260,18 @@ __device__ __forceinline__ unsigned v_lane(int lane) {
 template <typename T, int HD>
 __device__ __forceinline__ void scores(const Rows<HD> &w, unsigned k, floatx16 (&s)[2]) {
     using L = Lay<HD>;
+    i32x4 f[2][L::KS];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        s[j] = zero16();
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int ks = 0; ks < L::KS; ++ks)
-            s[j] = mfma32(*(lds_i32x4 *)(k ^ ((j * (HD / 8) + ks * 2) << 4)), w.q[j][ks], s[j], T());
-    }
+        for (int ks = 0; ks < L::KS; ++ks) f[j][ks] = *(lds_i32x4 *)(k ^ ((j * (HD / 8) + ks * 2) << 4));
+    __builtin_amdgcn_sched_barrier(0);   // all reads under way before the first product waits for one
+#pragma unroll
+    for (int j = 0; j < 2; ++j) s[j] = zero16();
+#pragma unroll
+    for (int ks = 0; ks < L::KS; ++ks)   // the maps in turn: a product does not wait for the one before it
+#pragma unroll
+        for (int j = 0; j < 2; ++j) s[j] = mfma32(f[j][ks], w.q[j][ks], s[j], T());
 }
 // scores of keys that the lane's row does not see: key 0 of the 32 at k0
 template <int HD>
@@ -276,42 +281,48 @@ __device__ __forceinline__ void mask_scores(const Rows<HD> &w, floatx16 (&s)[2],
     for (int r = 0; r < 16; ++r)
         if (16 * (r >> 3) + (r & 7) >= left) s[0][r] = s[1][r] = -INFINITY;
 }
-// Probabilities of 32 keys. The reference m moves only when a score passes it by more than 2^8: probabilities stay
-// below 2^8, inside f16, and most steps leave O as it is. Returns whether any lane's moved; al: by what O has to be
-// scaled before these probabilities' product is added.
-template <typename T, int HD>
-__device__ __forceinline__ bool probs(Rows<HD> &w, const floatx16 (&s)[2], i32x4 (&p)[2][2], float (&al)[2], float c) {
-    bool moved = false;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        float t = fmaxf(fmaxf(s[j][0], s[j][1]), s[j][2]);
-#pragma unroll
-        for (int r = 3; r < 15; r += 2) t = fmaxf(fmaxf(t, s[j][r]), s[j][r + 1]);
-        t = pair_max(fmaxf(t, s[j][15])) * c;
-        const bool up = t > w.m[j] + 8.0f;
-        const float mn = up ? t : w.m[j];
-        al[j] = __builtin_amdgcn_exp2f(w.m[j] - mn);
-        w.m[j] = mn;
-        moved |= up;
-        float sum = 0.0f;
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], c, -mn));
-            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r + 1], c, -mn));
-            sum += e0;
-            sum += e1;
-            p[j][r >> 3][(r & 7) >> 1] = pack2<T>(e0, e1);
-        }
-        w.l[j] = __builtin_fmaf(w.l[j], al[j], sum);
-    }
-    return __builtin_amdgcn_ballot_w64(moved) != 0;
+// sum + the two values of a register of probabilities: numerator and denominator see the same rounding
+__device__ __forceinline__ float dot_ones(int v, float sum, half_t) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, v), half2_t{1, 1}, sum, false);
 }
-template <int HD>
-__device__ __forceinline__ void rescale(Rows<HD> &w, const float (&al)[2]) {
+__device__ __forceinline__ float dot_ones(int v, float sum, bf16_t) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, v), bf16x2{1, 1}, sum, false);
+}
+// exp2(c s - m) of 16 scores, rounded, and their sum
+template <typename T>
+__device__ __forceinline__ float exp_scores(const floatx16 &s, float c, float m, i32x4 (&p)[2]) {
+    float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int r = 0; r < 16; r += 2) {
+        const int v = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -m)), __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], c, -m)));
+        p[r >> 3][(r & 7) >> 1] = v;
+        sum = dot_ones(v, sum, T());
+    }
+    return sum;
+}
+// Probabilities of 32 keys, to the reference m of earlier ones. A reference may lie below a score as long as no
+// probability nears f16's range: a lane's 16 add up to no more than 2^12. Only where one exceeds that (the first block:
+// m = -1e30) are the maxima taken, the references moved and O and the sums scaled; most blocks take no maximum at all.
+template <typename T, int HD>
+__device__ __forceinline__ void probs(Rows<HD> &w, const floatx16 (&s)[2], i32x4 (&p)[2][2], float c) {
+    float sum[2] = {exp_scores<T>(s[0], c, w.m[0], p[0]), exp_scores<T>(s[1], c, w.m[1], p[1])};
+    if (__builtin_amdgcn_ballot_w64(!(fmaxf(sum[0], sum[1]) <= 4096.0f)) != 0) {
 #pragma unroll
-        for (int d = 0; d < Lay<HD>::DT; ++d) w.o[j][d] *= al[j];
+        for (int j = 0; j < 2; ++j) {
+            float t = fmaxf(fmaxf(s[j][0], s[j][1]), s[j][2]);
+#pragma unroll
+            for (int r = 3; r < 15; r += 2) t = fmaxf(fmaxf(t, s[j][r]), s[j][r + 1]);
+            const float mn = fmaxf(w.m[j], pair_max(fmaxf(t, s[j][15])) * c);
+            const float al = __builtin_amdgcn_exp2f(w.m[j] - mn);
+            w.m[j] = mn;
+            w.l[j] *= al;
+#pragma unroll
+            for (int d = 0; d < Lay<HD>::DT; ++d) w.o[j][d] *= al;
+            sum[j] = exp_scores<T>(s[j], c, mn, p[j]);
+        }
+    }
+    w.l[0] += sum[0];
+    w.l[1] += sum[1];
 }
 // O^T += V^T P^T for 32 keys, v = v_lane + the V tile's address: A row = column 32d + (lane & 31) of V, keys
 // 16h + 8*(lane>>5) + 0..7 by two transposing reads of four
@@ -344,15 +355,12 @@ template <typename T, int HD>
 __device__ __forceinline__ void load_rows(Rows<HD> &w, const DiffAttnArgs &a, int b, int g, int G, int x, int nq, int nk, int lane) {
     using L = Lay<HD>;
     const RowOf ro = row_of(x, G);
-    const bool in = ro.qi < nq;
-    const T *q = (const T *)a.q + (long long)b * a.bsq + (long long)ro.qi * a.ldq + (g * G + ro.hg) * 2 * HD + 8 * (lane >> 5);
+    const bool in = ro.qi < nq;   // other lanes compute with query 0 and are not stored
+    const T *q = (const T *)a.q + (long long)b * a.bsq + (long long)(in ? ro.qi : 0) * a.ldq + (g * G + (in ? ro.hg : 0)) * 2 * HD + 8 * (lane >> 5);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
-        for (int ks = 0; ks < L::KS; ++ks) {
-            w.q[j][ks] = i32x4{0, 0, 0, 0};
-            if (in) w.q[j][ks] = *(const i32x4 *)(q + j * HD + ks * 16);
-        }
+        for (int ks = 0; ks < L::KS; ++ks) w.q[j][ks] = *(const i32x4 *)(q + j * HD + ks * 16);
         w.m[j] = -1e30f;
         w.l[j] = 0.0f;
 #pragma unroll
@@ -520,8 +528,6 @@ struct Attn {
         const int x0 = tile * 32 * RW;
         if (x0 / G >= nq) return;   // the whole workgroup: no row of the tile is there
         const int x = x0 + rw * 32 + (lane & 31);
-        Rows<HD> w;
-        load_rows<T, HD>(w, a, b, g, G, x, nq, nk, lane);
         // keys that any row of the tile and every row of the wave sees
         auto limit = [&](int xr) {
             const int qi = min(row_of(xr, G).qi, nq - 1);
@@ -541,13 +547,15 @@ struct Attn {
         const int end = min(u1, (keys + KB - 1) / KB);
         block_barrier();   // an earlier piece's LDS has been read
         if (u0 < end) issue(u0);
+        Rows<HD> w;
+        load_rows<T, HD>(w, a, b, g, G, x, nq, nk, lane);
         const RowOf ro = row_of(x, G);
         // values i of a lane are columns 32(i>>4) + 8((i&15)>>2) + 4*(lane>>5) + (i&3)
         const int i0 = kw * NQ, col0 = 32 * (i0 >> 4) + 2 * (i0 & 15) + 4 * (lane >> 5);
         float lam = 0.0f, nw[KW > 1 ? NQ : 1];
-        if constexpr (KW > 1) {   // few rows, where latency counts: loaded beside the first keys
-            if (piece < 0) {
-                lam = row_lambda(a, g, G, ro.hg, lane);
+        if (piece < 0) {   // loaded beside the first keys
+            lam = row_lambda(a, g, G, ro.hg, lane);
+            if constexpr (KW > 1) {
 #pragma unroll
                 for (int i = 0; i < NQ; ++i) nw[i] = a.norm_w ? a.norm_w[col0 + 32 * (i >> 4) + 8 * ((i & 15) >> 2) + (i & 3)] : 1.0f;
             }
@@ -563,10 +571,9 @@ struct Attn {
                 const int k0 = u * KB + 32 * blk;
                 floatx16 s[2];
                 i32x4 p[2][2];
-                float al[2];
                 scores<T, HD>(w, kl + at + blk * SUB, s);
                 if (k0 + 32 > all) mask_scores<HD>(w, s, k0, lane);
-                if (probs<T, HD>(w, s, p, al, c)) rescale<HD>(w, al);
+                probs<T, HD>(w, s, p, c);
                 product<T, HD>(w, vl + at + blk * SUB, p);
             }
         }
@@ -592,7 +599,6 @@ struct Attn {
                     *(float4 *)(to + j * 2 * HD + 32 * (i >> 4) + 2 * (i & 15)) = make_float4(o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]);
             return;
         }
-        if constexpr (KW == 1) lam = row_lambda(a, g, G, ro.hg, lane);
         const float r0 = l0 > 0.0f ? 1.0f / l0 : 0.0f, r1 = l1 > 0.0f ? lam / l1 : 0.0f;
         float ss = 0.0f;
 #pragma unroll
@@ -634,7 +640,7 @@ __device__ __forceinline__ Share shares(const DiffAttnArgs &a, const DiffPlan &p
 __device__ __forceinline__ int tile_order(const DiffAttnArgs &a, int heads, int i) { return a.causal ? heads - 1 - i : i; }   // the longest first
 
 template <typename T, int HD, int RW, int KW>
-__global__ __launch_bounds__(256, KW == 4 ? 1 : 2) void diff_attn_kernel(const DiffAttnArgs a, const DiffPlan pl) {
+__global__ __launch_bounds__(256, 2) void diff_attn_kernel(const DiffAttnArgs a, const DiffPlan pl) {
     using A = Attn<T, HD, RW, KW>;
     __shared__ __attribute__((aligned(1024))) char smem[A::LDS];
     const int lane = threadIdx.x & 63, nkv = (int)a.nkv;
