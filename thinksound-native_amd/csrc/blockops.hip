@@ -3,6 +3,8 @@
 // write it once.
 #include <math.h>
 
+#include <algorithm>
+
 #include "kernels.h"
 
 #include "dpp.h"
@@ -66,6 +68,102 @@ __global__ __launch_bounds__(256) void rope_axes_any_kernel(const RopeKernelArgs
         const float v0 = load_elem(a.x, a.dt, xr + h * a.hd + e0), v1 = load_elem(a.x, a.dt, xr + h * a.hd + e1);
         store_elem(a.y, a.dt, yr + h * a.hd + e0, turned ? v0 * cs - v1 * sn : v0);
         store_elem(a.y, a.dt, yr + h * a.hd + e1, turned ? v0 * sn + v1 * cs : v1);
+    }
+}
+
+// Whole 16-byte chunks: a workgroup takes rb rows, computes the cosines and sines of their pairs once (in LDS, for all
+// heads) while its first chunks are under way, and turns them. An item is a chunk (neighbouring pairs) or the two
+// chunks that hold a pair's halves; behind the axes a chunk is copied. per_head items a head, per_row a row;
+// the magic numbers divide by them.
+struct RopeChunks {
+    unsigned rb, per_head, per_row, head_magic, row_magic;
+};
+template <typename T, bool HALF>
+__global__ __launch_bounds__(256) void rope_axes_kernel(const RopeKernelArgs a, const RopeChunks c) {
+    constexpr int VE = 16 / sizeof(T), UN = HALF ? 4 : 8;   // elements of a chunk; items in flight a thread
+    typedef T vec __attribute__((ext_vector_type(VE)));
+    extern __shared__ float2 table[];   // [row of the workgroup][pair]
+    const unsigned np = a.hd / 2, r0 = blockIdx.x * c.rb, rows = min(c.rb, a.rows - r0), items = rows * c.per_row;
+    const T *x = (const T *)a.x + (long long)r0 * a.ldx;
+    T *y = (T *)a.y + (long long)r0 * a.ldy;
+    auto place = [&](unsigned i, unsigned &r, unsigned &h, unsigned &p, unsigned &e0, unsigned &e1) {   // item i: row, head, first pair, chunks
+        r = __umulhi(i, c.row_magic);
+        const unsigned in_row = i - r * c.per_row;
+        h = __umulhi(in_row, c.head_magic);
+        const unsigned k = (in_row - h * c.per_head) * VE;
+        if constexpr (HALF) {
+            unsigned axis;
+            p = k;
+            pair_at(a, p, axis, e0, e1);
+            if (2 * p >= a.total) {   // copied
+                p = MAX_PAIRS;
+                e0 = e1 = k + a.total / 2;
+            }
+        } else {
+            p = k / 2;
+            e0 = e1 = k;
+        }
+    };
+    auto fill = [&]() {
+        for (unsigned i = threadIdx.x; i < rows * np; i += 256) {
+            const unsigned r = i / np, p = i - r * np;
+            unsigned axis, e0, e1;
+            pair_at(a, p, axis, e0, e1);
+            float cs, sn;
+            turn(a.freq[p], a.pos[(long long)((r0 + r) % a.pos_rows) * a.n_axes + axis], cs, sn);
+            table[i] = make_float2(cs, sn);
+        }
+        __syncthreads();
+    };
+    for (unsigned i0 = 0; i0 < items; i0 += 256 * UN) {
+        vec v0[UN], v1[HALF ? UN : 1];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const unsigned i = i0 + u * 256 + threadIdx.x;
+            if (i >= items) break;
+            unsigned r, h, p, e0, e1;
+            place(i, r, h, p, e0, e1);
+            const T *row = x + (unsigned long long)r * a.ldx + h * a.hd;
+            v0[u] = *(const vec *)(row + e0);
+            if constexpr (HALF) v1[u] = *(const vec *)(row + e1);
+        }
+        if (i0 == 0) fill();
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const unsigned i = i0 + u * 256 + threadIdx.x;
+            if (i >= items) break;
+            unsigned r, h, p, e0, e1;
+            place(i, r, h, p, e0, e1);
+            T *row = y + (unsigned long long)r * a.ldy + h * a.hd;
+            const float2 *t = table + r * np;
+            if constexpr (HALF) {
+                if (p < MAX_PAIRS) {
+                    vec w0, w1;
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) {
+                        const float2 cs = t[p + e];
+                        const float f0 = (float)v0[u][e], f1 = (float)v1[u][e];
+                        w0[e] = (T)(f0 * cs.x - f1 * cs.y);
+                        w1[e] = (T)(f0 * cs.y + f1 * cs.x);
+                    }
+                    *(vec *)(row + e0) = w0;
+                    *(vec *)(row + e1) = w1;
+                } else {
+                    *(vec *)(row + e0) = v0[u];
+                }
+            } else {
+                vec w = v0[u];
+#pragma unroll
+                for (int e = 0; e < VE; e += 2) {
+                    if (e0 + e >= a.total) break;
+                    const float2 cs = t[p + e / 2];
+                    const float f0 = (float)v0[u][e], f1 = (float)v0[u][e + 1];
+                    w[e] = (T)(f0 * cs.x - f1 * cs.y);
+                    w[e + 1] = (T)(f0 * cs.y + f1 * cs.x);
+                }
+                *(vec *)(row + e0) = w;
+            }
+        }
     }
 }
 
@@ -154,6 +252,137 @@ __global__ __launch_bounds__(256) void gate_norm_any_kernel(const GateNormArgs a
     }
 }
 
+// Rows of H % 8 == 0 aligned elements: W waves a row, NC chunks of eight elements a lane, the row in registers between
+// one read and one write. A wave (a group of W) takes `per` rows one after the other and keeps what they share:
+// y = n(x_out) * A + B with A = pre_w (1 + scale), B = pre_b (1 + scale) + shift, and z's G = f_scale gate post_w, D =
+// f_scale gate post_b, made anew where a row of mod begins.
+template <typename TX, typename TF, int W, int NC>
+__global__ __launch_bounds__(W > 1 ? 64 * W : 256, W > 8 ? 4 : 2) void gate_norm_kernel(const GateNormArgs a, unsigned per) {
+    constexpr int GROUPS = W > 1 ? 1 : 4;   // row groups of a workgroup
+    __shared__ float red_all[GROUPS][W];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    float *red = red_all[wave / W];
+    const unsigned H = a.H, chunks = H / 8, first = (wave % W) * 64 + lane;
+    const unsigned group = blockIdx.x * GROUPS + wave / W;
+    const unsigned r0 = group * per, r1 = min(r0 + per, a.rows);
+    const float n = (float)H;
+    floatx8 A[NC], B[NC], G[NC], D[NC];
+    unsigned have = ~0u;
+    // sum over the row's waves; every wave of a workgroup takes part the same number of times (W > 1: one group)
+    auto row_sum = [&](float v) {
+        v = wave_sum(v);
+        if constexpr (W > 1) {
+            __syncthreads();
+            if (lane == 0) red[wave % W] = v;
+            __syncthreads();
+            v = red[0];
+#pragma unroll
+            for (int w = 1; w < W; ++w) v += red[w];
+        }
+        return v;
+    };
+    auto sum8 = [](const floatx8 &v) { return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])); };
+    // centres x for an LN, and its 1 / sqrt(mean square + eps)
+    auto norm = [&](floatx8 (&x)[NC], int kind, float eps) {
+        if (kind == NORM_NONE) return 1.0f;
+        float s = 0.0f;
+        if (kind == NORM_LN) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) s += sum8(x[c]);
+            const float mean = row_sum(s) / n;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                if (c * 64 * W + first < chunks) x[c] -= mean;
+            s = 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) s += sum8(x[c] * x[c]);
+        return 1.0f / sqrtf(row_sum(s) / n + eps);
+    };
+    for (unsigned r = r0; r < r1; ++r) {
+        floatx8 f[NC], x[NC];
+        typename Eight<TF>::type rf[NC];
+        typename Eight<TX>::type rx[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const unsigned k = c * 64 * W + first;
+            if (k < chunks) {
+                rf[c] = *(const typename Eight<TF>::type *)((const TF *)a.f + (unsigned long long)r * a.ldf + 8 * k);
+                rx[c] = *(const typename Eight<TX>::type *)((const TX *)a.x + (unsigned long long)r * a.ldx + 8 * k);
+            } else {
+                rf[c] = typename Eight<TF>::type{};
+                rx[c] = typename Eight<TX>::type{};
+            }
+        }
+        const unsigned m = r / a.mod_rows;
+        if (m != have) {
+            have = m;
+            const float *mod = a.mod ? a.mod + (unsigned long long)m * a.chunks * H : nullptr;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const unsigned k = min(c * 64 * W + first, chunks - 1);
+                auto vec = [&](const float *p, float other) {
+                    return p ? *(const floatx8 *)(p + 8 * k) : floatx8{other, other, other, other, other, other, other, other};
+                };
+                const floatx8 g = vec(a.gate >= 0 ? mod + (unsigned long long)a.gate * H : nullptr, 1.0f) * a.f_scale;
+                const floatx8 s = 1.0f + vec(a.scale >= 0 ? mod + (unsigned long long)a.scale * H : nullptr, 0.0f);
+                G[c] = g * vec(a.post_w, 1.0f);
+                D[c] = g * vec(a.post_b, 0.0f);
+                A[c] = s * vec(a.pre_w, 1.0f);
+                B[c] = s * vec(a.pre_b, 0.0f) + vec(a.shift >= 0 ? mod + (unsigned long long)a.shift * H : nullptr, 0.0f);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) f[c] = __builtin_convertvector(rf[c], floatx8);
+        const float inv = norm(f, a.post, a.post_eps);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const unsigned k = c * 64 * W + first;
+            x[c] = __builtin_convertvector(rx[c], floatx8) * a.x_scale + (f[c] * inv * G[c] + D[c]);
+            if (k < chunks) store8((TX *)a.x_out + (unsigned long long)r * a.ldo + 8 * k, x[c]);
+            else x[c] = floatx8{};
+        }
+        if (!a.y) continue;
+        const float pinv = norm(x, a.pre, a.pre_eps);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const unsigned k = c * 64 * W + first;
+            if (k >= chunks) break;
+            const floatx8 y = x[c] * pinv * A[c] + B[c];
+            const unsigned long long at = (unsigned long long)r * a.ldy + 8 * k;
+            if (a.ydt == DT_F32) store8((float *)a.y + at, y);
+            else if (a.ydt == DT_F16) store8((half_t *)a.y + at, y);
+            else store8((bf16_t *)a.y + at, y);
+        }
+    }
+}
+
+template <typename TX, typename TF, int W, int NC>
+int launch_gate_norm_rows(const GateNormArgs &a, hipStream_t st) {
+    constexpr unsigned GROUPS = W > 1 ? 1 : 4;
+    // rows in turn only where they share a row of mod and every CU still has sixteen waves
+    const unsigned waves = a.rows * W / (256 * 16);
+    const unsigned per = std::max(1u, std::min({waves, a.mod_rows, 8u}));
+    const unsigned groups = (a.rows + per - 1) / per;
+    TSN_LAUNCH((gate_norm_kernel<TX, TF, W, NC>), dim3((groups + GROUPS - 1) / GROUPS), dim3(W > 1 ? 64 * W : 256), 0, st, a, per);
+    TSN_HIP_CHECK(hipGetLastError());
+    return TSN_OK;
+}
+template <typename TX, typename TF>
+int launch_gate_norm_typed(const GateNormArgs &a, hipStream_t st) {
+    if (a.H <= 512) return launch_gate_norm_rows<TX, TF, 1, 1>(a, st);
+    if (a.H <= 1024) return launch_gate_norm_rows<TX, TF, 1, 2>(a, st);
+    if (a.H <= 2048) return launch_gate_norm_rows<TX, TF, 2, 2>(a, st);
+    if (a.H <= 4096) return launch_gate_norm_rows<TX, TF, 4, 2>(a, st);
+    if (a.H <= 8192) return launch_gate_norm_rows<TX, TF, 8, 2>(a, st);
+    return launch_gate_norm_rows<TX, TF, 16, 2>(a, st);
+}
+template <typename TX>
+int launch_gate_norm_f(const GateNormArgs &a, hipStream_t st) {
+    if (a.fdt == DT_F32) return launch_gate_norm_typed<TX, float>(a, st);
+    return a.fdt == DT_F16 ? launch_gate_norm_typed<TX, half_t>(a, st) : launch_gate_norm_typed<TX, bf16_t>(a, st);
+}
+
 } // namespace
 
 int rope_axes_check(RopeAxesArgs &a) {
@@ -198,6 +427,39 @@ int launch_rope_axes(const RopeAxesArgs &c, hipStream_t st) {
             a.freq[a.total / 2 + p] = c.inverse ? -f : f;
         }
         a.total += c.dim[i];
+    }
+    // whole chunks: aligned rows and heads, and for halves whole chunks of each half
+    const unsigned ve = c.dt == DT_F32 ? 4 : 8;
+    bool whole = (((uintptr_t)c.x | (uintptr_t)c.y) & 15) == 0 && c.ldx % ve == 0 && c.ldy % ve == 0 && c.hd % ve == 0;
+    if (c.half_split)
+        for (unsigned i = 0; i < c.n_axes; ++i) whole = whole && c.dim[i] % (2 * ve) == 0;
+    if (whole) {
+        RopeChunks k{};
+        k.per_head = c.half_split ? (a.total / 2 + (c.hd - a.total)) / ve : c.hd / ve;
+        k.per_row = c.nh * k.per_head;
+        const unsigned un = c.half_split ? 4 : 8;
+        // rows that give a workgroup's threads `un` items each, but no more than leave every CU eight workgroups
+        const unsigned long long fill = c.rows / 2048 + 1;
+        k.rb = (unsigned)std::max<unsigned long long>(1, std::min<unsigned long long>({256 * un / k.per_row, fill, 16384 / c.hd}));
+        // i / d = umulhi(i, magic) while i * d < 2^32
+        auto magic = [](unsigned d) { return d == 1 ? 0u : (unsigned)((0x100000000ULL + d - 1) / d); };
+        k.head_magic = magic(k.per_head);
+        k.row_magic = magic(k.per_row);
+        const unsigned long long most = (unsigned long long)k.rb * k.per_row;
+        whole = k.per_head > 1 && most * k.per_row < (1ULL << 32);
+        if (whole) {
+            const dim3 grid((c.rows + k.rb - 1) / k.rb);
+            const size_t lds = (size_t)k.rb * (c.hd / 2) * sizeof(float2);
+#define ROPE(T)                                                                                     \
+    if (c.half_split) TSN_LAUNCH((rope_axes_kernel<T, true>), grid, dim3(256), lds, st, a, k);      \
+    else TSN_LAUNCH((rope_axes_kernel<T, false>), grid, dim3(256), lds, st, a, k)
+            if (c.dt == DT_F32) { ROPE(float); }
+            else if (c.dt == DT_F16) { ROPE(half_t); }
+            else { ROPE(bf16_t); }
+#undef ROPE
+            TSN_HIP_CHECK(hipGetLastError());
+            return TSN_OK;
+        }
     }
     const unsigned long long n = (unsigned long long)c.rows * (c.hd / 2);
     TSN_LAUNCH(rope_axes_any_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
@@ -253,6 +515,12 @@ int gate_add_norm_check(GateNormArgs &a) {
 }
 
 int launch_gate_add_norm(const GateNormArgs &a, hipStream_t st) {
+    const uintptr_t at = (uintptr_t)a.x | (uintptr_t)a.f | (uintptr_t)a.x_out | (uintptr_t)a.y | (uintptr_t)a.mod | (uintptr_t)a.post_w |
+                         (uintptr_t)a.post_b | (uintptr_t)a.pre_w | (uintptr_t)a.pre_b;
+    if (a.H % 8 == 0 && ((a.ldx | a.ldf | a.ldo | a.ldy) & 7) == 0 && (at & 31) == 0) {
+        if (a.xdt == DT_F32) return launch_gate_norm_f<float>(a, st);
+        return a.xdt == DT_F16 ? launch_gate_norm_f<half_t>(a, st) : launch_gate_norm_f<bf16_t>(a, st);
+    }
     TSN_LAUNCH(gate_norm_any_kernel, dim3(a.rows), dim3(256), a.H * sizeof(float), st, a);
     TSN_HIP_CHECK(hipGetLastError());
     return TSN_OK;

@@ -22,6 +22,18 @@ __device__ __forceinline__ void store_elem(void *p, int dt, long long i, float v
     else ((bf16_t *)p)[i] = (bf16_t)v;
 }
 
+// eight elements at a 16-byte aligned place (f32: 32 bytes from it)
+typedef float floatx8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8_e __attribute__((ext_vector_type(8)));
+template <typename T> struct Eight;
+template <> struct Eight<float> { typedef floatx8 type; };
+template <> struct Eight<half_t> { typedef half8 type; };
+template <> struct Eight<bf16_t> { typedef bf16x8_e type; };
+template <typename T>
+__device__ __forceinline__ void store8(T *p, const floatx8 &v) {
+    *(typename Eight<T>::type *)p = __builtin_convertvector(v, typename Eight<T>::type);
+}
+
 // rows of `width` bytes, `ld` bytes apart, in samples `bs` bytes apart
 struct Window {
     const void *p;
