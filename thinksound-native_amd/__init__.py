@@ -141,6 +141,13 @@ class RopeAxesSpec(ctypes.Structure):
                 ("n_axes", ctypes.c_uint32), ("dim", ctypes.c_uint32 * 4), ("base", ctypes.c_float * 4),
                 ("fscale", ctypes.c_float * 4), ("half_split", ctypes.c_int), ("inverse", ctypes.c_int)]
 
+    def sizes(self):
+        """(array, bytes, optional) of x, pos, y"""
+        n, size = self.nh * self.hd, 4 if self.dtype == F32 else 2
+        return (("x", _span(self.rows, self.ldx or n, n) * size, False),
+                ("pos", (self.pos_rows or self.rows) * self.n_axes * 4, False),
+                ("y", _span(self.rows, self.ldy or n, n) * size, False))
+
 
 class DiffAttnSpec(ctypes.Structure):
     """tsn_diff_attn_spec (include/tsn.h)."""
@@ -151,6 +158,14 @@ class DiffAttnSpec(ctypes.Structure):
                 ("lam_heads", ctypes.c_uint32), ("causal", ctypes.c_int), ("scale", ctypes.c_float),
                 ("lambda_init", ctypes.c_float), ("eps", ctypes.c_float)]
 
+    def sizes(self):
+        """(array, bytes, optional) of q, k, v, out, lam, norm_w, q_len, kv_len"""
+        B, Sq, Sk, hd = self.B, self.Sq, self.Sk, self.hd
+        wq, wk = 2 * self.nh * hd, 2 * self.nkv * hd
+        return (("q", 2 * _span3(B, Sq, self.ldq or wq, self.bsq, wq), False), ("k", 2 * _span3(B, Sk, self.ldk or wk, self.bsk, wk), False),
+                ("v", 2 * _span3(B, Sk, self.ldv or wk, self.bsv, wk), False), ("out", 2 * _span3(B, Sq, self.ldo or wq, self.bso, wq), False),
+                ("lam", 16 * self.lam_heads * hd, False), ("norm_w", 8 * hd, True), ("q_len", 4 * B, True), ("kv_len", 4 * B, True))
+
 
 class GateNormSpec(ctypes.Structure):
     """tsn_gate_norm_spec (include/tsn.h)."""
@@ -160,6 +175,15 @@ class GateNormSpec(ctypes.Structure):
                 ("x_scale", ctypes.c_float), ("f_scale", ctypes.c_float), ("chunks", ctypes.c_uint32),
                 ("mod_rows", ctypes.c_uint32), ("gate", ctypes.c_int), ("shift", ctypes.c_int), ("scale", ctypes.c_int),
                 ("post_eps", ctypes.c_float), ("pre_eps", ctypes.c_float)]
+
+    def sizes(self):
+        """(array, bytes, optional) of x, f, x_out, y, mod, post_w, post_b, pre_w, pre_b"""
+        rows, H, m = self.rows, self.H, self.mod_rows
+        sx, sf, sy = (4 if dt == F32 else 2 for dt in (self.x_dtype, self.f_dtype, self.y_dtype))
+        return (("x", _span(rows, self.ldx or H, H) * sx, False), ("f", _span(rows, self.ldf or H, H) * sf, False),
+                ("x_out", _span(rows, self.ldo or H, H) * sx, False), ("y", _span(rows, self.ldy or H, H) * sy, True),
+                ("mod", (-(-rows // m) if m else 1) * self.chunks * H * 4, True), ("post_w", 4 * H, True),
+                ("post_b", 4 * H, True), ("pre_w", 4 * H, True), ("pre_b", 4 * H, True))
 
 
 class KernelStat(ctypes.Structure):
@@ -994,33 +1018,17 @@ class Runtime:
     # --- block operators: device arrays, and a spec made once (rope_axes_spec, diff_attn_spec, gate_norm_spec) ---
     def rope_axes(self, spec, x, pos, y):
         """multi-axis rotary positions of the heads in x's rows, to y (which may be x)"""
-        rows, size = spec.rows, 4 if spec.dtype == F32 else 2
-        n = spec.nh * spec.hd
-        _hold("rope_axes", (("x", x, _span(rows, spec.ldx or n, n) * size),
-                            ("pos", pos, (spec.pos_rows or rows) * spec.n_axes * 4),
-                            ("y", y, _span(rows, spec.ldy or n, n) * size)))
+        _hold("rope_axes", spec, (x, pos, y))
         call("tsn_rope_axes", self.h, spec, x.p, pos.p, y.p)
 
     def diff_attention(self, spec, q, k, v, lam, norm_w, q_len, kv_len, out):
         """differential attention; norm_w, q_len and kv_len may be None"""
-        B, Sq, Sk, hd = spec.B, spec.Sq, spec.Sk, spec.hd
-        wq, wk = 2 * spec.nh * hd, 2 * spec.nkv * hd
-        _hold("diff_attention", (("q", q, 2 * _span3(B, Sq, spec.ldq or wq, spec.bsq, wq)),
-                                 ("k", k, 2 * _span3(B, Sk, spec.ldk or wk, spec.bsk, wk)),
-                                 ("v", v, 2 * _span3(B, Sk, spec.ldv or wk, spec.bsv, wk)),
-                                 ("out", out, 2 * _span3(B, Sq, spec.ldo or wq, spec.bso, wq)),
-                                 ("lam", lam, 16 * spec.lam_heads * hd)),
-              (("norm_w", norm_w, 8 * hd), ("q_len", q_len, 4 * B), ("kv_len", kv_len, 4 * B)))
+        _hold("diff_attention", spec, (q, k, v, out, lam, norm_w, q_len, kv_len))
         call("tsn_diff_attention", self.h, spec, q.p, k.p, v.p, lam.p, _p(norm_w), _p(q_len), _p(kv_len), out.p)
 
     def gate_add_norm(self, spec, x, f, mod, x_out, y, post_w=None, post_b=None, pre_w=None, pre_b=None):
         """x_out = x_scale*x + f_scale*gate*post(f), y = pre(x_out)*(1 + scale) + shift; y and mod may be None"""
-        rows, H, m = spec.rows, spec.H, spec.mod_rows
-        sx, sf, sy = (4 if dt == F32 else 2 for dt in (spec.x_dtype, spec.f_dtype, spec.y_dtype))
-        _hold("gate_add_norm", (("x", x, _span(rows, spec.ldx or H, H) * sx), ("f", f, _span(rows, spec.ldf or H, H) * sf),
-                                ("x_out", x_out, _span(rows, spec.ldo or H, H) * sx)),
-              (("y", y, _span(rows, spec.ldy or H, H) * sy), ("mod", mod, (-(-rows // m) if m else 1) * spec.chunks * H * 4),
-               ("post_w", post_w, 4 * H), ("post_b", post_b, 4 * H), ("pre_w", pre_w, 4 * H), ("pre_b", pre_b, 4 * H)))
+        _hold("gate_add_norm", spec, (x, f, x_out, y, mod, post_w, post_b, pre_w, pre_b))
         call("tsn_gate_add_norm", self.h, spec, x.p, f.p, _p(mod), _p(post_w), _p(post_b), _p(pre_w), _p(pre_b), x_out.p,
              _p(y))
 
@@ -1063,13 +1071,17 @@ def _need(what, arr, numel, itemsize=4, optional=False):
         raise ValueError("%s: %d bytes needed, the array holds %d" % (what, numel * itemsize, have))
 
 
-def _hold(what, arrays, optional=()):
-    """_need of several (name, array, bytes); the optional ones may be None"""
-    for name, arr, nbytes in arrays:
-        if arr is None or getattr(arr, "nbytes", -1) < nbytes or not hasattr(arr, "p"):
-            _need("%s: %s" % (what, name), arr, nbytes, 1)
-    for name, arr, nbytes in optional:
-        if arr is not None and (getattr(arr, "nbytes", -1) < nbytes or not hasattr(arr, "p")):
+def _hold(what, spec, arrays):
+    """_need of a block operator's arrays, in the order of the spec's sizes(); the spec keeps them until a field changes"""
+    key = bytes(spec)
+    kept = getattr(spec, "_kept", None)
+    if kept is None or kept[0] != key:
+        kept = spec._kept = key, spec.sizes()
+    for arr, (name, nbytes, optional) in zip(arrays, kept[1]):
+        if arr is None:
+            if not optional:
+                raise ValueError("%s: %s: a device array is required" % (what, name))
+        elif type(arr) is not DeviceArray and not hasattr(arr, "p") or arr.nbytes < nbytes:
             _need("%s: %s" % (what, name), arr, nbytes, 1)
 
 

@@ -257,7 +257,7 @@ __global__ __launch_bounds__(256) void gate_norm_any_kernel(const GateNormArgs a
 // y = n(x_out) * A + B with A = pre_w (1 + scale), B = pre_b (1 + scale) + shift, and z's G = f_scale gate post_w, D =
 // f_scale gate post_b, made anew where a row of mod begins.
 template <typename TX, typename TF, int W, int NC>
-__global__ __launch_bounds__(W > 1 ? 64 * W : 256, W > 8 ? 4 : 2) void gate_norm_kernel(const GateNormArgs a, unsigned per) {
+__global__ __launch_bounds__(W > 1 ? 64 * W : 256, 2) void gate_norm_kernel(const GateNormArgs a, unsigned per) {
     constexpr int GROUPS = W > 1 ? 1 : 4;   // row groups of a workgroup
     __shared__ float red_all[GROUPS][W];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -299,10 +299,9 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256, W > 8 ? 4 : 2) void gate_norm
         for (int c = 0; c < NC; ++c) s += sum8(x[c] * x[c]);
         return 1.0f / sqrtf(row_sum(s) / n + eps);
     };
-    for (unsigned r = r0; r < r1; ++r) {
-        floatx8 f[NC], x[NC];
-        typename Eight<TF>::type rf[NC];
-        typename Eight<TX>::type rx[NC];
+    typename Eight<TF>::type rf[NC];
+    typename Eight<TX>::type rx[NC];
+    auto load = [&](unsigned r) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const unsigned k = c * 64 * W + first;
@@ -314,6 +313,10 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256, W > 8 ? 4 : 2) void gate_norm
                 rx[c] = typename Eight<TX>::type{};
             }
         }
+    };
+    if (r0 < r1) load(r0);
+    for (unsigned r = r0; r < r1; ++r) {
+        floatx8 f[NC], x[NC];
         const unsigned m = r / a.mod_rows;
         if (m != have) {
             have = m;
@@ -333,12 +336,16 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256, W > 8 ? 4 : 2) void gate_norm
             }
         }
 #pragma unroll
-        for (int c = 0; c < NC; ++c) f[c] = __builtin_convertvector(rf[c], floatx8);
+        for (int c = 0; c < NC; ++c) {
+            f[c] = __builtin_convertvector(rf[c], floatx8);
+            x[c] = __builtin_convertvector(rx[c], floatx8) * a.x_scale;
+        }
+        if (r + 1 < r1) load(r + 1);   // under way while this row is worked on
         const float inv = norm(f, a.post, a.post_eps);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const unsigned k = c * 64 * W + first;
-            x[c] = __builtin_convertvector(rx[c], floatx8) * a.x_scale + (f[c] * inv * G[c] + D[c]);
+            x[c] += f[c] * inv * G[c] + D[c];
             if (k < chunks) store8((TX *)a.x_out + (unsigned long long)r * a.ldo + 8 * k, x[c]);
             else x[c] = floatx8{};
         }
@@ -360,9 +367,10 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256, W > 8 ? 4 : 2) void gate_norm
 template <typename TX, typename TF, int W, int NC>
 int launch_gate_norm_rows(const GateNormArgs &a, hipStream_t st) {
     constexpr unsigned GROUPS = W > 1 ? 1 : 4;
-    // rows in turn only where they share a row of mod and every CU still has sixteen waves
-    const unsigned waves = a.rows * W / (256 * 16);
-    const unsigned per = std::max(1u, std::min({waves, a.mod_rows, 8u}));
+    // Rows that share a row of mod in turn, so that the waves fill the device once (eight a CU): 6352 rows of 1024 take
+    // 22.2 us a row a wave, 16.6 us four rows a wave (4.7 TB/s). A row of mod of its own: a row a wave.
+    const unsigned waves = (unsigned)(((unsigned long long)a.rows * W + 2047) / 2048);
+    const unsigned per = a.mod_rows == 1 ? 1 : std::min(waves, 32u);
     const unsigned groups = (a.rows + per - 1) / per;
     TSN_LAUNCH((gate_norm_kernel<TX, TF, W, NC>), dim3((groups + GROUPS - 1) / GROUPS), dim3(W > 1 ? 64 * W : 256), 0, st, a, per);
     TSN_HIP_CHECK(hipGetLastError());
@@ -374,8 +382,7 @@ int launch_gate_norm_typed(const GateNormArgs &a, hipStream_t st) {
     if (a.H <= 1024) return launch_gate_norm_rows<TX, TF, 1, 2>(a, st);
     if (a.H <= 2048) return launch_gate_norm_rows<TX, TF, 2, 2>(a, st);
     if (a.H <= 4096) return launch_gate_norm_rows<TX, TF, 4, 2>(a, st);
-    if (a.H <= 8192) return launch_gate_norm_rows<TX, TF, 8, 2>(a, st);
-    return launch_gate_norm_rows<TX, TF, 16, 2>(a, st);
+    return launch_gate_norm_rows<TX, TF, 8, 2>(a, st);   // to 8192
 }
 template <typename TX>
 int launch_gate_norm_f(const GateNormArgs &a, hipStream_t st) {
@@ -517,7 +524,7 @@ int gate_add_norm_check(GateNormArgs &a) {
 int launch_gate_add_norm(const GateNormArgs &a, hipStream_t st) {
     const uintptr_t at = (uintptr_t)a.x | (uintptr_t)a.f | (uintptr_t)a.x_out | (uintptr_t)a.y | (uintptr_t)a.mod | (uintptr_t)a.post_w |
                          (uintptr_t)a.post_b | (uintptr_t)a.pre_w | (uintptr_t)a.pre_b;
-    if (a.H % 8 == 0 && ((a.ldx | a.ldf | a.ldo | a.ldy) & 7) == 0 && (at & 31) == 0) {
+    if (a.H % 8 == 0 && a.H <= 8192 && ((a.ldx | a.ldf | a.ldo | a.ldy) & 7) == 0 && (at & 31) == 0) {
         if (a.xdt == DT_F32) return launch_gate_norm_f<float>(a, st);
         return a.xdt == DT_F16 ? launch_gate_norm_f<half_t>(a, st) : launch_gate_norm_f<bf16_t>(a, st);
     }
