@@ -477,15 +477,14 @@ __device__ __forceinline__ Part part_at(const DiffAttnArgs &a, const DiffPlan &p
 }
 
 // A workgroup's worker: 128 rows, 32 a wave. The four waves share K and V tiles of 64 keys, two stages in LDS: the next is
-// loaded while one is worked on. Two workgroups a CU, one's matrix products cover the other's softmax.
+// loaded while one is worked on. Two workgroups a CU (hd 32: three), one's matrix products cover the other's softmax.
 template <typename T, int HD>
 struct Wide {
     using L = Lay<HD>;
     static constexpr int TR = 128, KB = 64;
     static constexpr int OP = KB * L::ROW, STAGE = 2 * OP, SUB = 32 * L::ROW;
     static constexpr int NB = OP / 1024 / 4;         // 1 KB blocks of K, of V, a wave and unit
-    static constexpr int NO = L::DT * 16;            // products of a lane and map
-    static constexpr int LDS = 2 * STAGE;
+    static constexpr int LDS = 2 * STAGE, WAVES = HD == 32 ? 3 : 2;
 
     // units of a tile; a piece of it (to the workspace) or, piece < 0, all of it
     static __device__ __forceinline__ void run(const DiffAttnArgs &a, const DiffPlan &pl, char *smem, const Part &t, int piece) {
@@ -610,7 +609,7 @@ struct Few {
     static constexpr int KS = HD / 32, DT = 2 * HD / 16;   // MFMA steps of a map's width; 16-column tiles of V
     static constexpr int OP = 32 * L::ROW, NB = OP / 1024; // a wave's K (V) tile and its 1 KB blocks
     static constexpr int NO = DT * 4, NQ = NO / 4;         // products of a lane and map; those that it has after the merge
-    static constexpr int LDS = 8 * OP + 4 * 64 * 5 * 4;
+    static constexpr int LDS = 8 * OP + 4 * 64 * 5 * 4, WAVES = HD == 32 ? 3 : 2;
     static_assert(4 * 2 * NO * 256 <= 8 * OP, "the products fit in the tiles");
     // the 16 K rows of a read differ in bits 0, 1, 3, 4, the 8 V rows of half a wave in bits 0, 1, 3 (32 bytes each)
     static __device__ __forceinline__ int ksw(int r) {
@@ -856,15 +855,27 @@ __device__ __forceinline__ Share shares(const DiffAttnArgs &a, const DiffPlan &p
 }
 
 template <typename T, int HD, typename A>
-__global__ __launch_bounds__(256, 2) void diff_attn_kernel(const DiffAttnArgs a, const DiffPlan pl) {
+__global__ __launch_bounds__(256, A::WAVES) void diff_attn_kernel(const DiffAttnArgs a, const DiffPlan pl) {
     __shared__ __attribute__((aligned(1024))) char smem[A::LDS];
     const int lane = threadIdx.x & 63, nkv = (int)a.nkv;
     if ((int)blockIdx.x < pl.full) {
-        const int t = (int)xcd_remap(blockIdx.x, pl.full), bg = t / pl.ntile;
+        // workgroups go round the 8 XCDs in turn. A head's tiles stay on one, for its L2; heads go round too, so that a
+        // short sample's are not all on one; causal tiles the longest first, over all the XCD's heads
+        const int heads = nkv * (int)a.B;
+        int bg, i;
+        if (heads % 8 == 0 && pl.full == pl.tiles) {
+            const int per = heads / 8, idx = (int)blockIdx.x >> 3;
+            i = a.causal ? idx / per : idx % pl.ntile;
+            bg = (a.causal ? idx - i * per : idx / pl.ntile) * 8 + ((int)blockIdx.x & 7);
+        } else {
+            const int t = (int)xcd_remap(blockIdx.x, pl.full);
+            bg = t / pl.ntile;
+            i = t - bg * pl.ntile;
+        }
         Part p;
         p.b = bg / nkv;
         p.g = bg - p.b * nkv;
-        p.tile = tile_order(a, pl.ntile, t - bg * pl.ntile);
+        p.tile = tile_order(a, pl.ntile, i);
         p.nq = q_rows(a, p.b);
         p.nk = kv_rows(a, p.b);
         p.u0 = 0;
@@ -1019,7 +1030,7 @@ DiffChoice choose(const DiffAttnArgs &a) {
     const double h = a.hd == 64 ? 1.0 : 0.55;
     const double stream = (double)heads * a.Sk * 8 * a.hd / 5.5e6;   // K and V from memory
     const double seen = a.causal && a.Sq > a.Sk / 2 ? 0.55 : 1.0;    // of the keys, by many rows
-    const double ragged = a.kv_len ? 0.8 : 1.0;                      // a guess: a longer tile makes no one wait when shared
+    const double ragged = a.kv_len && rows <= 16 ? 0.8 : 1.0;        // a guess: a longer cache makes no one wait when shared
     DiffChoice best{};
     double least = 1e300;
     for (int tr : {128, 16}) {

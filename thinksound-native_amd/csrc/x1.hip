@@ -4,8 +4,8 @@
 // One pass over the keys: each map keeps its running maximum, sum and product with V (the online
 // softmax), and the two are joined once both sums are known.
 #include <math.h>
-#include <stdio.h>
-#include <stdlib.h>
+
+#include <algorithm>
 
 #include "kernels.h"
 
@@ -260,13 +260,18 @@ __device__ __forceinline__ unsigned v_lane(int lane) {
 template <typename T, int HD>
 __device__ __forceinline__ void scores(const Rows<HD> &w, unsigned k, floatx16 (&s)[2]) {
     using L = Lay<HD>;
+    i32x4 f[2][L::KS];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        s[j] = zero16();
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int ks = 0; ks < L::KS; ++ks)
-            s[j] = mfma32(*(lds_i32x4 *)(k ^ ((j * (HD / 8) + ks * 2) << 4)), w.q[j][ks], s[j], T());
-    }
+        for (int ks = 0; ks < L::KS; ++ks) f[j][ks] = *(lds_i32x4 *)(k ^ ((j * (HD / 8) + ks * 2) << 4));
+    __builtin_amdgcn_sched_barrier(0);   // all reads under way before the first product waits for one
+#pragma unroll
+    for (int j = 0; j < 2; ++j) s[j] = zero16();
+#pragma unroll
+    for (int ks = 0; ks < L::KS; ++ks)   // the maps in turn: a product does not wait for the one before it
+#pragma unroll
+        for (int j = 0; j < 2; ++j) s[j] = mfma32(f[j][ks], w.q[j][ks], s[j], T());
 }
 // scores of keys that the lane's row does not see: key 0 of the 32 at k0
 template <int HD>
@@ -276,42 +281,48 @@ __device__ __forceinline__ void mask_scores(const Rows<HD> &w, floatx16 (&s)[2],
     for (int r = 0; r < 16; ++r)
         if (16 * (r >> 3) + (r & 7) >= left) s[0][r] = s[1][r] = -INFINITY;
 }
-// Probabilities of 32 keys. The reference m moves only when a score passes it by more than 2^8: probabilities stay
-// below 2^8, inside f16, and most steps leave O as it is. Returns whether any lane's moved; al: by what O has to be
-// scaled before these probabilities' product is added.
-template <typename T, int HD>
-__device__ __forceinline__ bool probs(Rows<HD> &w, const floatx16 (&s)[2], i32x4 (&p)[2][2], float (&al)[2], float c) {
-    bool moved = false;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        float t = fmaxf(fmaxf(s[j][0], s[j][1]), s[j][2]);
-#pragma unroll
-        for (int r = 3; r < 15; r += 2) t = fmaxf(fmaxf(t, s[j][r]), s[j][r + 1]);
-        t = pair_max(fmaxf(t, s[j][15])) * c;
-        const bool up = t > w.m[j] + 8.0f;
-        const float mn = up ? t : w.m[j];
-        al[j] = __builtin_amdgcn_exp2f(w.m[j] - mn);
-        w.m[j] = mn;
-        moved |= up;
-        float sum = 0.0f;
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], c, -mn));
-            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r + 1], c, -mn));
-            sum += e0;
-            sum += e1;
-            p[j][r >> 3][(r & 7) >> 1] = pack2<T>(e0, e1);
-        }
-        w.l[j] = __builtin_fmaf(w.l[j], al[j], sum);
-    }
-    return __builtin_amdgcn_ballot_w64(moved) != 0;
+// sum + the two values of a register of probabilities: numerator and denominator see the same rounding
+__device__ __forceinline__ float dot_ones(int v, float sum, half_t) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, v), half2_t{1, 1}, sum, false);
 }
-template <int HD>
-__device__ __forceinline__ void rescale(Rows<HD> &w, const float (&al)[2]) {
+__device__ __forceinline__ float dot_ones(int v, float sum, bf16_t) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, v), bf16x2{1, 1}, sum, false);
+}
+// exp2(c s - m) of 16 scores, rounded, and their sum
+template <typename T>
+__device__ __forceinline__ float exp_scores(const floatx16 &s, float c, float m, i32x4 (&p)[2]) {
+    float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int r = 0; r < 16; r += 2) {
+        const int v = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -m)), __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], c, -m)));
+        p[r >> 3][(r & 7) >> 1] = v;
+        sum = dot_ones(v, sum, T());
+    }
+    return sum;
+}
+// Probabilities of 32 keys, to the reference m of earlier ones. A reference may lie below a score as long as no
+// probability nears f16's range: a lane's 16 add up to no more than 2^12. Only where one exceeds that (the first block:
+// m = -1e30) are the maxima taken, the references moved and O and the sums scaled; most blocks take no maximum at all.
+template <typename T, int HD>
+__device__ __forceinline__ void probs(Rows<HD> &w, const floatx16 (&s)[2], i32x4 (&p)[2][2], float c) {
+    float sum[2] = {exp_scores<T>(s[0], c, w.m[0], p[0]), exp_scores<T>(s[1], c, w.m[1], p[1])};
+    if (__builtin_amdgcn_ballot_w64(!(fmaxf(sum[0], sum[1]) <= 4096.0f)) != 0) {
 #pragma unroll
-        for (int d = 0; d < Lay<HD>::DT; ++d) w.o[j][d] *= al[j];
+        for (int j = 0; j < 2; ++j) {
+            float t = fmaxf(fmaxf(s[j][0], s[j][1]), s[j][2]);
+#pragma unroll
+            for (int r = 3; r < 15; r += 2) t = fmaxf(fmaxf(t, s[j][r]), s[j][r + 1]);
+            const float mn = fmaxf(w.m[j], pair_max(fmaxf(t, s[j][15])) * c);
+            const float al = __builtin_amdgcn_exp2f(w.m[j] - mn);
+            w.m[j] = mn;
+            w.l[j] *= al;
+#pragma unroll
+            for (int d = 0; d < Lay<HD>::DT; ++d) w.o[j][d] *= al;
+            sum[j] = exp_scores<T>(s[j], c, mn, p[j]);
+        }
+    }
+    w.l[0] += sum[0];
+    w.l[1] += sum[1];
 }
 // O^T += V^T P^T for 32 keys, v = v_lane + the V tile's address: A row = column 32d + (lane & 31) of V, keys
 // 16h + 8*(lane>>5) + 0..7 by two transposing reads of four
@@ -344,15 +355,12 @@ template <typename T, int HD>
 __device__ __forceinline__ void load_rows(Rows<HD> &w, const DiffAttnArgs &a, int b, int g, int G, int x, int nq, int nk, int lane) {
     using L = Lay<HD>;
     const RowOf ro = row_of(x, G);
-    const bool in = ro.qi < nq;
-    const T *q = (const T *)a.q + (long long)b * a.bsq + (long long)ro.qi * a.ldq + (g * G + ro.hg) * 2 * HD + 8 * (lane >> 5);
+    const bool in = ro.qi < nq;   // other lanes compute with query 0 and are not stored
+    const T *q = (const T *)a.q + (long long)b * a.bsq + (long long)(in ? ro.qi : 0) * a.ldq + (g * G + (in ? ro.hg : 0)) * 2 * HD + 8 * (lane >> 5);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
-        for (int ks = 0; ks < L::KS; ++ks) {
-            w.q[j][ks] = i32x4{0, 0, 0, 0};
-            if (in) w.q[j][ks] = *(const i32x4 *)(q + j * HD + ks * 16);
-        }
+        for (int ks = 0; ks < L::KS; ++ks) w.q[j][ks] = *(const i32x4 *)(q + j * HD + ks * 16);
         w.m[j] = -1e30f;
         w.l[j] = 0.0f;
 #pragma unroll
@@ -372,95 +380,128 @@ __device__ __forceinline__ float row_lambda(const DiffAttnArgs &a, int g, int G,
     return lam;
 }
 
-// How a launch's work is cut. A tile is the 32*RW rows x0.. of one key/value head of one sample, its keys are `units`
-// units of Lay::KB keys. The first `full` tiles have a workgroup each; the units of the others, one after the other, are
-// shared out evenly among `shared` workgroups, whose pieces of tiles go to ws and are joined by diff_attn_join_kernel.
+// How a launch's work is cut. A tile is TR rows of one key/value head of one sample, its keys are units of KB. The first
+// `full` tiles have a workgroup each. The units of the others, one after the other, are shared out evenly among `shared`
+// workgroups; their pieces of tiles go to the workspace and are joined by diff_attn_join_kernel. A piece's place there is
+// its workgroup's number plus its tile's: both only grow along the units, and one of them does at every cut.
 struct DiffPlan {
-    int ntile;       // tiles of a key/value head
-    int tiles;       // of all
-    int units;       // key units of a tile
+    int ntile;          // tiles of a key/value head
+    int tiles, units;   // of all heads and samples; of a tile (by Sk)
     int full, shared;
-    float *o;        // [piece][row of the tile][map][2 HD]: products with V, not divided
-    float4 *st;      // [piece][row of the tile]: reference and sum of each map
+    int by_len;         // full = 0 and lengths are given: the units are counted by them
+    float *o;           // [piece][row of the tile][map][2 HD]: products with V, not divided
+    float4 *st;         // [piece][row of the tile]: reference and sum of each map
 };
-// unit range of shared workgroup p, and the piece that it and tile t (counted from the first shared one) have in common:
-// both only grow along the units, so p + t is a number of its own
-__host__ __device__ __forceinline__ long long share_begin(const DiffPlan &pl, int p) {
-    return (long long)(pl.tiles - pl.full) * pl.units * p / pl.shared;
+struct Share {   // shared workgroup p's units begin at p*q + min(p, r)
+    unsigned q, r;
+    __device__ __forceinline__ unsigned begin(unsigned p) const { return p * q + min(p, r); }
+    __device__ __forceinline__ unsigned holder(unsigned u) const { return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q; }
+};
+// The samples' units by their lengths, 64 samples at a time: lane i looks at sample b0 + i, which has nkv * tiles * n
+// units (tiles of a head, units of a tile)
+template <int TR, int KB>
+struct ByLen {
+    int b0, nq, nk, tiles;
+    unsigned n, own, upto;   // units of the lane's sample, and up to and with it of the 64
+    __device__ __forceinline__ void look(const DiffAttnArgs &a, int from, int lane) {
+        b0 = from;
+        const int b = min(from + lane, (int)a.B - 1);
+        nq = q_rows(a, b);
+        nk = kv_rows(a, b);
+        tiles = (int)(((unsigned)nq * (a.nh / a.nkv) + TR - 1) / TR);
+        n = (unsigned)max(1, (nk + KB - 1) / KB);
+        own = from + lane < (int)a.B ? a.nkv * tiles * n : 0;
+        unsigned v = own;   // sum over the lanes up to this one: within rows of 16, then from row to row
+        v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+        upto = v;
+    }
+    __device__ __forceinline__ unsigned all() const { return __builtin_amdgcn_readlane(upto, 63); }
+    // of all samples; the first 64 are being looked at before and after
+    __device__ __forceinline__ unsigned total(const DiffAttnArgs &a, int lane) {
+        unsigned t = all();
+        for (int from = 64; from < (int)a.B; from += 64) {
+            ByLen x;
+            x.look(a, from, lane);
+            t += x.all();
+        }
+        return t;
+    }
+};
+// A tile and some of its units
+struct Part {
+    int b, g, tile, nq, nk, u0, u1, n, place;   // n: units of the tile; place: the tile's number among all (static)
+};
+__device__ __forceinline__ int tile_order(const DiffAttnArgs &a, int heads, int i) { return a.causal ? heads - 1 - i : i; }   // the longest first
+// unit u and what follows it in its tile, up to unit end
+template <int TR, int KB>
+__device__ __forceinline__ Part part_at(const DiffAttnArgs &a, const DiffPlan &pl, const ByLen<TR, KB> &first64, unsigned u, unsigned end, int lane) {
+    Part p;
+    int heads = pl.ntile, in_sample;
+    if (pl.by_len) {
+        ByLen<TR, KB> x = first64;
+        unsigned before = 0;
+        while (u >= before + x.all() && x.b0 + 64 < (int)a.B) {
+            before += x.all();
+            x.look(a, x.b0 + 64, lane);
+        }
+        const int i = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(before + x.upto > u)) - 1;
+        p.b = x.b0 + i;
+        p.nq = __builtin_amdgcn_readlane(x.nq, i);
+        p.nk = __builtin_amdgcn_readlane(x.nk, i);
+        p.n = __builtin_amdgcn_readlane(x.n, i);
+        heads = __builtin_amdgcn_readlane(x.tiles, i);
+        const unsigned in = u - before - __builtin_amdgcn_readlane(x.upto - x.own, i);
+        in_sample = (int)(in / (unsigned)p.n);
+        p.u0 = (int)(in - in_sample * (unsigned)p.n);
+        p.g = in_sample / heads;
+    } else {
+        const int ts = (int)(u / (unsigned)pl.units), t = pl.full + ts, bg = t / pl.ntile;
+        p.u0 = (int)(u - (unsigned)ts * pl.units);
+        p.n = pl.units;
+        p.b = bg / (int)a.nkv;
+        p.g = bg - p.b * (int)a.nkv;
+        p.nq = q_rows(a, p.b);
+        p.nk = kv_rows(a, p.b);
+        in_sample = t - p.b * (int)a.nkv * pl.ntile;
+    }
+    const int i = in_sample - p.g * heads;
+    p.tile = tile_order(a, heads, i);
+    p.u1 = (int)min((unsigned)p.n, p.u0 + (end - u));
+    p.place = (p.b * (int)a.nkv + p.g) * pl.ntile + tile_order(a, pl.ntile, p.tile) - pl.full;
+    return p;
 }
 
-// One tile or piece of one: 32 rows a wave, RW waves side by side; KW waves share the rows of one and take every KW-th
-// block of 32 keys, and are merged at the end through LDS. All four read the same K and V tiles, two stages in LDS: the
-// next is loaded while one is worked on. Two workgroups a CU (KW = 4: one): one's matrix products cover the other's
-// softmax.
-template <typename T, int HD, int RW, int KW>
-struct Attn {
+// A workgroup's worker: 128 rows, 32 a wave. The four waves share K and V tiles of 64 keys, two stages in LDS: the next is
+// loaded while one is worked on. Two workgroups a CU, one's matrix products cover the other's softmax.
+template <typename T, int HD>
+struct Wide {
     using L = Lay<HD>;
-    static constexpr int NSUB = KW > 2 ? KW : 2;     // blocks of 32 keys in a unit
-    static constexpr int KB = 32 * NSUB;
+    static constexpr int TR = 128, KB = 64;
     static constexpr int OP = KB * L::ROW, STAGE = 2 * OP, SUB = 32 * L::ROW;
     static constexpr int NB = OP / 1024 / 4;         // 1 KB blocks of K, of V, a wave and unit
-    static constexpr int NO = 2 * L::DT * 16;        // products of a lane
-    static constexpr int MERGE = KW > 1 ? RW * (KW / 2) * 64 * 4 * (NO + 4) : 0;
-    static constexpr int LDS = 2 * STAGE > MERGE ? 2 * STAGE : MERGE;
-    static_assert(RW * KW == 4, "four waves");
+    static constexpr int NO = L::DT * 16;            // products of a lane and map
+    static constexpr int LDS = 2 * STAGE;
 
-    static __device__ __forceinline__ void merge(Rows<HD> &w, float *buf, int rw, int kw, int lane) {
-#pragma unroll
-        for (int half = KW / 2; half > 0; half /= 2) {
-            // lane's values 64 floats apart: no bank conflicts
-            float *p = buf + ((kw % half) * RW + rw) * 64 * (NO + 4) + lane;
-            block_barrier();   // the key tiles, or the previous round's values, have been read
-            if (kw >= half && kw < 2 * half) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                    for (int d = 0; d < L::DT; ++d)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) p[((j * L::DT + d) * 16 + r) * 64] = w.o[j][d][r];
-                    p[(NO + 2 * j) * 64] = w.m[j];
-                    p[(NO + 2 * j + 1) * 64] = w.l[j];
-                }
-            }
-            block_barrier();
-            if (kw < half) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float m2 = p[(NO + 2 * j) * 64], l2 = p[(NO + 2 * j + 1) * 64];
-                    const float mn = fmaxf(w.m[j], m2);
-                    const float a1 = __builtin_amdgcn_exp2f(w.m[j] - mn), a2 = __builtin_amdgcn_exp2f(m2 - mn);
-                    w.m[j] = mn;
-                    w.l[j] = w.l[j] * a1 + l2 * a2;
-#pragma unroll
-                    for (int d = 0; d < L::DT; ++d)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) w.o[j][d][r] = w.o[j][d][r] * a1 + p[((j * L::DT + d) * 16 + r) * 64] * a2;
-                }
-            }
-        }
-    }
-
-    static __device__ __forceinline__ void run(const DiffAttnArgs &a, const DiffPlan &pl, char *smem, int t, int u0, int u1, int piece) {
+    // units of a tile; a piece of it (to the workspace) or, piece < 0, all of it
+    static __device__ __forceinline__ void run(const DiffAttnArgs &a, const DiffPlan &pl, char *smem, const Part &t, int piece) {
         const unsigned lds = (unsigned)(unsigned long)(lds_char *)smem;
         const int lane = threadIdx.x & 63;
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const int rw = wave % RW, kw = wave / RW;
-        const int bg = t / pl.ntile, in_head = t - bg * pl.ntile;
-        const int tile = a.causal ? pl.ntile - 1 - in_head : in_head;   // causal: the longest first
-        const int b = bg / (int)a.nkv, g = bg - b * (int)a.nkv, G = (int)(a.nh / a.nkv);
-        const int nq = q_rows(a, b), nk = kv_rows(a, b);
-        const int x0 = tile * 32 * RW;
+        const int b = t.b, g = t.g, G = (int)(a.nh / a.nkv), nq = t.nq, nk = t.nk;
+        const int x0 = t.tile * TR;
         if (x0 / G >= nq) return;   // the whole workgroup: no row of the tile is there
-        const int x = x0 + rw * 32 + (lane & 31);
-        Rows<HD> w;
-        load_rows<T, HD>(w, a, b, g, G, x, nq, nk, lane);
-        // keys that any row of the tile, any row of the wave, and every row of the wave sees
+        const int x = x0 + wave * 32 + (lane & 31);
+        // keys that any row of the tile and every row of the wave sees
         auto limit = [&](int xr) {
             const int qi = min(row_of(xr, G).qi, nq - 1);
             return a.causal ? min(nk, max(0, qi + nk - nq + 1)) : nk;
         };
-        const int keys = limit(x0 + 32 * RW - 1), all = limit(x0 + rw * 32);
-        const int wkeys = row_of(x0 + rw * 32, G).qi < nq ? limit(x0 + rw * 32 + 31) : 0;
+        const int keys = limit(x0 + TR - 1), all = limit(x0 + wave * 32);
         const char *kp = (const char *)((const T *)a.k + (long long)b * a.bsk + g * 2 * HD);
         const char *vp = (const char *)((const T *)a.v + (long long)b * a.bsv + g * 2 * HD);
         const unsigned ldk = a.ldk * 2, ldv = a.ldv * 2;
@@ -471,48 +512,46 @@ struct Attn {
             load_tile<HD, NB>(lo, kp + k0 * ldk, vp + k0 * ldv, ldk, ldv, min(KB, nk - u * KB), lds + (u & 1) * STAGE + wave * NB * 1024, OP);
         };
         const float c = a.scale > 0.0f ? a.scale * LOG2E : 1e-30f;   // a scale of 0 must not meet a masked score's infinity
-        const int end = min(u1, (keys + KB - 1) / KB);
+        const int end = min(t.u1, (keys + KB - 1) / KB);
         block_barrier();   // an earlier piece's LDS has been read
-        if (u0 < end) issue(u0);
-        for (int u = u0; u < end; ++u) {
+        if (t.u0 < end) issue(t.u0);
+        Rows<HD> w;
+        load_rows<T, HD>(w, a, b, g, G, x, nq, nk, lane);
+        const RowOf ro = row_of(x, G);
+        const float lam = piece < 0 ? row_lambda(a, g, G, ro.hg, lane) : 0.0f;   // loaded beside the first keys
+        for (int u = t.u0; u < end; ++u) {
             wait_vmcnt<0>();
             block_barrier();
             if (u + 1 < end) issue(u + 1);
             const unsigned at = (u & 1) * STAGE;
 #pragma unroll 1
-            for (int i = 0; i < NSUB / KW; ++i) {
-                const int blk = i * KW + kw;
-                const int k0 = u * KB + 32 * blk;
-
+            for (int i = 0; i < KB / 32; ++i) {
+                const int k0 = u * KB + 32 * i;
                 floatx16 s[2];
                 i32x4 p[2][2];
-                float al[2];
-                scores<T, HD>(w, kl + at + blk * SUB, s);
+                scores<T, HD>(w, kl + at + i * SUB, s);
                 if (k0 + 32 > all) mask_scores<HD>(w, s, k0, lane);
-                if (probs<T, HD>(w, s, p, al, c)) rescale<HD>(w, al);
-                product<T, HD>(w, vl + at + blk * SUB, p);
+                probs<T, HD>(w, s, p, c);
+                product<T, HD>(w, vl + at + i * SUB, p);
             }
         }
-        if constexpr (KW > 1) merge(w, (float *)smem, rw, kw, lane);
-        if (kw > 0) return;
-        const RowOf ro = row_of(x, G);
         const float l0 = pair_sum(w.l[0]), l1 = pair_sum(w.l[1]);
+        // value r of tile d is column 32d + 8(r>>2) + 4*(lane>>5) + (r&3)
+        const int col0 = 4 * (lane >> 5);
         if (piece >= 0) {
             if (ro.qi >= nq) return;
-            const long long row = (long long)piece * (32 * RW) + rw * 32 + (lane & 31);
+            const long long row = (long long)piece * TR + wave * 32 + (lane & 31);
             if (lane < 32) pl.st[row] = make_float4(w.m[0], l0, w.m[1], l1);
-            float *o = pl.o + row * (4 * HD) + 4 * (lane >> 5);
+            float *to = pl.o + row * (4 * HD) + col0;
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int d = 0; d < L::DT; ++d)
 #pragma unroll
-                    for (int q4 = 0; q4 < 4; ++q4)
-                        *(float4 *)(o + j * 2 * HD + 32 * d + 8 * q4) = make_float4(w.o[j][d][4 * q4], w.o[j][d][4 * q4 + 1],
-                                                                                   w.o[j][d][4 * q4 + 2], w.o[j][d][4 * q4 + 3]);
+                    for (int r = 0; r < 16; r += 4)
+                        *(float4 *)(to + j * 2 * HD + 32 * d + 2 * r) = make_float4(w.o[j][d][r], w.o[j][d][r + 1], w.o[j][d][r + 2], w.o[j][d][r + 3]);
             return;
         }
-        const float lam = row_lambda(a, g, G, ro.hg, lane);
         const float r0 = l0 > 0.0f ? 1.0f / l0 : 0.0f, r1 = l1 > 0.0f ? lam / l1 : 0.0f;
         float ss = 0.0f;
 #pragma unroll
@@ -525,96 +564,389 @@ struct Attn {
             }
         ss = pair_sum(ss);
         if (ro.qi >= nq) return;
-        const float f = a.norm_w ? (1.0f - a.lambda_init) / sqrtf(ss / (float)(2 * HD) + a.eps) : 1.0f;
-        T *out = (T *)a.out + (long long)b * a.bso + (long long)ro.qi * a.ldo + (g * G + ro.hg) * 2 * HD;
+        if (a.norm_w) {
+            const float f = (1.0f - a.lambda_init) / sqrtf(ss / (float)(2 * HD) + a.eps);
+            const float *nw = a.norm_w + col0;
+#pragma unroll
+            for (int d = 0; d < L::DT; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) w.o[0][d][r] = w.o[0][d][r] * f * nw[32 * d + 8 * (r >> 2) + (r & 3)];
+        }
+        T *out = (T *)a.out + (long long)b * a.bso + (long long)ro.qi * a.ldo + (g * G + ro.hg) * 2 * HD + col0;
 #pragma unroll
         for (int d = 0; d < L::DT; ++d)
 #pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-                const int col = 32 * d + 8 * q4 + 4 * (lane >> 5);
-                float y[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    y[e] = w.o[0][d][4 * q4 + e];
-                    if (a.norm_w) y[e] = y[e] * f * a.norm_w[col + e];
-                }
-                *(int2 *)(out + col) = make_int2(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]));
-            }
+            for (int r = 0; r < 16; r += 4)
+                *(int2 *)(out + 32 * d + 2 * r) = make_int2(pack2<T>(w.o[0][d][r], w.o[0][d][r + 1]), pack2<T>(w.o[0][d][r + 2], w.o[0][d][r + 3]));
     }
 };
 
-template <typename T, int HD, int RW, int KW>
-__global__ __launch_bounds__(256, KW == 4 ? 1 : 2) void diff_attn_kernel(const DiffAttnArgs a, const DiffPlan pl) {
-    using A = Attn<T, HD, RW, KW>;
-    __shared__ __attribute__((aligned(1024))) char smem[A::LDS];
-    const unsigned wg = xcd_remap(blockIdx.x, gridDim.x);
-    int t = (int)wg, u0 = 0, u1 = pl.units, piece = -1;
-    long long u = 0, end = 0;   // a shared workgroup's units that are still to do
-    const int p = (int)wg - pl.full;
-    if (p >= 0) {
-        u = share_begin(pl, p);
-        end = share_begin(pl, p + 1);
-    }
-    do {
-        if (p >= 0) {
-            if (u >= end) return;
-            const int ts = (int)(u / pl.units);
-            u0 = (int)(u - (long long)ts * pl.units);
-            u1 = (int)min((long long)pl.units, u0 + (end - u));
-            u += u1 - u0;
-            t = pl.full + ts;
-            piece = u0 == 0 && u1 == pl.units ? -1 : p + ts;
-        }
-        A::run(a, pl, smem, t, u0, u1, piece);
-    } while (p >= 0);
+// A workgroup's worker for few rows: 16, the same in all four waves. Wave w takes keys 32w.. of every unit of 128, which it
+// alone reads: it loads them into LDS of its own and waits for nothing but its own loads, K of the next unit under way
+// as soon as this one's is in registers, V likewise. The waves' products are merged at the end through LDS.
+// 16x16x32 MFMA (A row and B column = lane & 15, K group g = lane >> 4, D[4g + r][lane & 15], r = 0..3), operands as in
+// the wide kernel: row i of the two products over 32 keys' K takes keys 8(i>>2) + (i&3) and 4 more, so that a lane has
+// keys 8g + 0..7 of query lane & 15.
+typedef floatx4 f32x4;
+__device__ __forceinline__ f32x4 mfma16(i32x4 a, i32x4 b, f32x4 c, half_t) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
 }
-
-// Joins the pieces of the shared tiles: HD/2 lanes a row, four columns of each map a lane, pieces in the order of
-// their keys.
+__device__ __forceinline__ f32x4 mfma16(i32x4 a, i32x4 b, f32x4 c, bf16_t) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// the four lanes of a query (l, l ^ 16, l ^ 32, l ^ 48) get the maximum, the sum
+__device__ __forceinline__ float quad_max(float v) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return pair_max(fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1])));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return pair_sum(__uint_as_float(p[0]) + __uint_as_float(p[1]));
+}
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs a, const DiffPlan pl, int rows_tile) {
-    constexpr int LR = HD / 2, RPW = 256 / LR;
-    const int lane = threadIdx.x & (LR - 1);
-    const long long id = (long long)blockIdx.x * RPW + threadIdx.x / LR;
-    const int ts = (int)(id / rows_tile), r = (int)(id - (long long)ts * rows_tile);
-    if (ts >= pl.tiles - pl.full) return;
-    // the shared workgroups that hold the tile's first and last unit
-    const long long first = (long long)ts * pl.units, last = first + pl.units - 1;
-    const long long U = (long long)(pl.tiles - pl.full) * pl.units;
-    auto holder = [&](long long u) {
-        int p = (int)(u * pl.shared / U);
-        while (share_begin(pl, p + 1) <= u) ++p;
-        while (share_begin(pl, p) > u) --p;
-        return p;
-    };
-    const int p0 = holder(first), p1 = holder(last);
-    if (p0 == p1) return;   // in one piece: written already
-    const int t = pl.full + ts, bg = t / pl.ntile, in_head = t - bg * pl.ntile;
-    const int tile = a.causal ? pl.ntile - 1 - in_head : in_head;
-    const int b = bg / (int)a.nkv, g = bg - b * (int)a.nkv, G = (int)(a.nh / a.nkv);
-    const RowOf ro = row_of(tile * rows_tile + r, G);
-    if (ro.qi >= q_rows(a, b)) return;
-    const int h = g * G + ro.hg;
-    float m[2] = {-1e30f, -1e30f}, l[2] = {0.0f, 0.0f};
-    for (int p = p0; p <= p1; ++p) {
-        const float4 st = pl.st[(long long)(p + ts) * rows_tile + r];
-        m[0] = fmaxf(m[0], st.x);
-        m[1] = fmaxf(m[1], st.z);
+struct Few {
+    using L = Lay<HD>;
+    static constexpr int TR = 16, KB = 128;
+    static constexpr int KS = HD / 32, DT = 2 * HD / 16;   // MFMA steps of a map's width; 16-column tiles of V
+    static constexpr int OP = 32 * L::ROW, NB = OP / 1024; // a wave's K (V) tile and its 1 KB blocks
+    static constexpr int NO = DT * 4, NQ = NO / 4;         // products of a lane and map; those that it has after the merge
+    static constexpr int LDS = 8 * OP + 4 * 64 * 5 * 4;
+    static_assert(4 * 2 * NO * 256 <= 8 * OP, "the products fit in the tiles");
+    // the 16 K rows of a read differ in bits 0, 1, 3, 4, the 8 V rows of half a wave in bits 0, 1, 3 (32 bytes each)
+    static __device__ __forceinline__ int ksw(int r) {
+        return HD == 64 ? (r & 3) | ((r >> 3) & 3) << 2 : ((r >> 1) & 1) | ((r >> 3) & 3) << 1;
     }
-    float o[2][4] = {};
-    for (int p = p0; p <= p1; ++p) {
-        const long long row = (long long)(p + ts) * rows_tile + r;
-        const float4 st = pl.st[row];
-        const float w[2] = {__builtin_amdgcn_exp2f(st.x - m[0]), __builtin_amdgcn_exp2f(st.z - m[1])};
-        l[0] += st.y * w[0];
-        l[1] += st.w * w[1];
+    static __device__ __forceinline__ int vsw(int r) {
+        return HD == 64 ? ((r & 3) | ((r >> 3) & 1) << 2) << 1 : (((r >> 1) & 1) | ((r >> 3) & 1) << 1) << 1;
+    }
+
+    static __device__ __forceinline__ float exps(const f32x4 (&s)[2], float c, float m, i32x4 &p) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) {
+                const int v = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[h][r], c, -m)), __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][r + 1], c, -m)));
+                p[2 * h + r / 2] = v;
+                sum = dot_ones(v, sum, T());
+            }
+        return sum;
+    }
+
+    static __device__ __forceinline__ void run(const DiffAttnArgs &a, const DiffPlan &pl, char *smem, const Part &t, int piece) {
+        const int lane = threadIdx.x & 63, g4 = lane >> 4, l16 = lane & 15;
+        const int kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int b = t.b, g = t.g, G = (int)(a.nh / a.nkv), nq = t.nq, nk = t.nk;
+        const int x0 = t.tile * TR;
+        if (x0 / G >= nq) return;   // the whole workgroup: no row of the tile is there
+        const RowOf ro = row_of(x0 + l16, G);
+        const bool in = ro.qi < nq;   // other lanes compute with query 0 and are not stored
+        auto limit = [&](int qi) { return a.causal ? min(nk, max(0, qi + nk - nq + 1)) : nk; };
+        const int keys = limit(min(row_of(x0 + TR - 1, G).qi, nq - 1)), all = limit(row_of(x0, G).qi);
+        const int lim = in ? limit(ro.qi) : 0;
+        const int end = min(t.u1, (keys + KB - 1) / KB);
+        // the wave's tiles, and the lane's share of their loads
+        const unsigned sk = (unsigned)(unsigned long)(lds_char *)smem + kw * 2 * OP, sv = sk + OP;
+        const char *kp = (const char *)((const T *)a.k + (long long)b * a.bsk + g * 2 * HD);
+        const char *vp = (const char *)((const T *)a.v + (long long)b * a.bsv + g * 2 * HD);
+        const unsigned ldk = a.ldk * 2, ldv = a.ldv * 2;
+        const int lr = lane / L::CPR, lc = lane % L::CPR;
+        unsigned ok[NB], ov[NB];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int r = lr + i * L::RPB;
+            ok[i] = (unsigned)r * ldk + ((lc ^ ksw(r)) << 4);
+            ov[i] = (unsigned)r * ldv + ((lc ^ vsw(r)) << 4);
+        }
+        auto load = [&](int u, const char *p, unsigned ld, const unsigned (&o)[NB], unsigned to) {
+            const int k0 = u * KB + 32 * kw, n = min(32, nk - k0) - 1;   // rows behind the last key read as zero
+            const i32x4 rs = buffer(p + (long long)k0 * ld, n < 0 ? 0u : (unsigned)n * ld + L::ROW);
+#pragma unroll
+            for (int i = 0; i < NB; ++i) dma16(rs, o[i], 0, to + i * 1024);
+        };
+        wait_vmcnt<0>();   // an earlier piece's stores are not counted among the loads below
+        block_barrier();   // its LDS has been read
+        if (t.u0 < end) {
+            load(t.u0, kp, ldk, ok, sk);
+            load(t.u0, vp, ldv, ov, sv);
+        }
+        const T *q = (const T *)a.q + (long long)b * a.bsq + (long long)(in ? ro.qi : 0) * a.ldq + (g * G + (in ? ro.hg : 0)) * 2 * HD + 8 * g4;
+        i32x4 qf[2][KS];
+        f32x4 o[2][DT];
+        float m[2] = {-1e30f, -1e30f}, l[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const float4 v = *(const float4 *)(pl.o + row * (4 * HD) + j * 2 * HD + 4 * lane);
-            o[j][0] += v.x * w[j];
-            o[j][1] += v.y * w[j];
-            o[j][2] += v.z * w[j];
-            o[j][3] += v.w * w[j];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) qf[j][ks] = *(const i32x4 *)(q + j * HD + ks * 32);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[j][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        // after the merge value i of the wave's is column 16*(d0 + i/4) + 4*g4 + i%4
+        const int col0 = 16 * (DT / 4) * kw + 4 * g4;
+        float lam = 0.0f, nw[NQ];
+        if (piece < 0) {
+            lam = row_lambda(a, g, G, ro.hg, lane);
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) nw[i] = a.norm_w ? a.norm_w[col0 + 16 * (i >> 2) + (i & 3)] : 1.0f;
+        }
+        const float c = a.scale > 0.0f ? a.scale * LOG2E : 1e-30f;   // a scale of 0 must not meet a masked score's infinity
+        // K row 8*(l16>>2) + (l16&3), chunk g4; V row 8*g4 + (l16>>2), column 4*(l16&3)
+        const int kr = 8 * (l16 >> 2) + (l16 & 3), vr = 8 * g4 + (l16 >> 2);
+        const unsigned kl = sk + kr * L::ROW + ((g4 ^ ksw(kr)) << 4);
+        const unsigned vl = sv + vr * L::ROW + ((((l16 & 3) >> 1) ^ vsw(vr)) << 4) + (l16 & 1) * 8;
+        asm volatile("" ::: "memory");
+        for (int u = t.u0; u < end; ++u) {
+            const bool more = u + 1 < end;
+            wait_vmcnt<NB>();   // K is there; V's NB blocks may still be under way
+            i32x4 kf[2][2][KS];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) kf[j][h][ks] = *(lds_i32x4 *)((kl ^ ((j * (HD / 8) + ks * 4) << 4)) + 4 * h * L::ROW);
+            __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt 0: the tile is in registers
+            asm volatile("" ::: "memory");
+            if (more) load(u + 1, kp, ldk, ok, sk);
+            f32x4 s[2][2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) s[j][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) s[j][h] = mfma16(kf[j][h][ks], qf[j][ks], s[j][h], T());
+            const int k0 = u * KB + 32 * kw;
+            if (k0 + 32 > all) {
+                const int left = lim - k0 - 8 * g4;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (4 * h + r >= left) s[0][h][r] = s[1][h][r] = -INFINITY;
+            }
+            i32x4 p[2];
+            float sum[2] = {exps(s[0], c, m[0], p[0]), exps(s[1], c, m[1], p[1])};
+            if (__builtin_amdgcn_ballot_w64(!(fmaxf(sum[0], sum[1]) <= 4096.0f)) != 0) {   // as in probs
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float top = fmaxf(fmaxf(fmaxf(s[j][0][0], s[j][0][1]), fmaxf(s[j][0][2], s[j][0][3])),
+                                            fmaxf(fmaxf(s[j][1][0], s[j][1][1]), fmaxf(s[j][1][2], s[j][1][3])));
+                    const float mn = fmaxf(m[j], quad_max(top) * c);
+                    const float al = __builtin_amdgcn_exp2f(m[j] - mn);
+                    m[j] = mn;
+                    l[j] *= al;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) o[j][d] *= al;
+                    sum[j] = exps(s[j], c, mn, p[j]);
+                }
+            }
+            l[0] += sum[0];
+            l[1] += sum[1];
+            if (more) wait_vmcnt<NB>();   // V is there; the next K's NB blocks may still be under way
+            else wait_vmcnt<0>();
+            i32x4 vf[DT];
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const unsigned vd = vl ^ (d << 5);
+                const int2 lo = __builtin_bit_cast(int2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)vd));
+                const int2 hi = __builtin_bit_cast(int2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vd + 4 * L::ROW)));
+                vf[d] = i32x4{lo.x, lo.y, hi.x, hi.y};
+            }
+            __builtin_amdgcn_s_waitcnt(0xC07F);
+            asm volatile("" ::: "memory");
+            if (more) load(u + 1, vp, ldv, ov, sv);
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) o[j][d] = mfma16(vf[d], p[j], o[j][d], T());
+        }
+        // every wave leaves its products in LDS (a lane's four are 16 bytes, lanes next to each other) and takes a quarter of all
+        float4 *prod = (float4 *)smem + lane;
+        float4 *st = (float4 *)(smem + 8 * OP) + lane;
+        block_barrier();   // the tiles have been read
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) prod[(kw * 2 * DT + j * DT + d) * 64] = make_float4(o[j][d][0], o[j][d][1], o[j][d][2], o[j][d][3]);
+        st[kw * 64] = make_float4(m[0], quad_sum(l[0]), m[1], quad_sum(l[1]));
+        block_barrier();
+        float f[2][4], y[2][NQ];
+        m[0] = m[1] = -1e30f;
+        l[0] = l[1] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float4 v = st[k * 64];
+            m[0] = fmaxf(m[0], v.x);
+            m[1] = fmaxf(m[1], v.z);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float4 v = st[k * 64];
+            f[0][k] = __builtin_amdgcn_exp2f(v.x - m[0]);
+            f[1][k] = __builtin_amdgcn_exp2f(v.z - m[1]);
+            l[0] += v.y * f[0][k];
+            l[1] += v.w * f[1][k];
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < NQ; i += 4) {
+                float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float4 v = prod[(k * 2 * DT + j * DT + kw * (DT / 4) + i / 4) * 64];
+                    s.x += v.x * f[j][k];
+                    s.y += v.y * f[j][k];
+                    s.z += v.z * f[j][k];
+                    s.w += v.w * f[j][k];
+                }
+                y[j][i] = s.x;
+                y[j][i + 1] = s.y;
+                y[j][i + 2] = s.z;
+                y[j][i + 3] = s.w;
+            }
+        if (piece >= 0) {
+            if (!in) return;
+            const long long row = (long long)piece * TR + l16;
+            if (g4 == 0 && kw == 0) pl.st[row] = make_float4(m[0], l[0], m[1], l[1]);
+            float *to = pl.o + row * (4 * HD) + col0;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < NQ; i += 4) *(float4 *)(to + j * 2 * HD + 4 * i) = make_float4(y[j][i], y[j][i + 1], y[j][i + 2], y[j][i + 3]);
+            return;
+        }
+        const float r0 = l[0] > 0.0f ? 1.0f / l[0] : 0.0f, r1 = l[1] > 0.0f ? lam / l[1] : 0.0f;
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            y[0][i] = y[0][i] * r0 - y[1][i] * r1;
+            ss += y[0][i] * y[0][i];
+        }
+        if (a.norm_w) {   // the row's squares over the waves, in their order
+            float *red = (float *)(smem + 8 * OP + 4 * 64 * 16) + lane;
+            red[kw * 64] = quad_sum(ss);
+            block_barrier();
+            ss = ((red[0] + red[64]) + red[128]) + red[192];
+            const float fn = (1.0f - a.lambda_init) / sqrtf(ss / (float)(2 * HD) + a.eps);
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) y[0][i] = y[0][i] * fn * nw[i];
+        }
+        if (!in) return;
+        T *out = (T *)a.out + (long long)b * a.bso + (long long)ro.qi * a.ldo + (g * G + ro.hg) * 2 * HD + col0;
+#pragma unroll
+        for (int i = 0; i < NQ; i += 4)
+            *(int2 *)(out + 4 * i) = make_int2(pack2<T>(y[0][i], y[0][i + 1]), pack2<T>(y[0][i + 2], y[0][i + 3]));
+    }
+};
+
+template <int TR, int KB>
+__device__ __forceinline__ Share shares(const DiffAttnArgs &a, const DiffPlan &pl, ByLen<TR, KB> &x, int lane) {
+    unsigned U = (unsigned)(pl.tiles - pl.full) * pl.units;
+    if (pl.by_len) {
+        x.look(a, 0, lane);
+        U = x.total(a, lane);
+    }
+    const unsigned q = U / (unsigned)pl.shared;
+    return Share{q, U - q * pl.shared};
+}
+
+template <typename T, int HD, typename A>
+__global__ __launch_bounds__(256, HD == 32 ? 3 : 2) void diff_attn_kernel(const DiffAttnArgs a, const DiffPlan pl) {
+    __shared__ __attribute__((aligned(1024))) char smem[A::LDS];
+    const int lane = threadIdx.x & 63, nkv = (int)a.nkv;
+    if ((int)blockIdx.x < pl.full) {
+        const int t = (int)xcd_remap(blockIdx.x, pl.full), bg = t / pl.ntile;
+        Part p;
+        p.b = bg / nkv;
+        p.g = bg - p.b * nkv;
+        p.tile = tile_order(a, pl.ntile, t - bg * pl.ntile);
+        p.nq = q_rows(a, p.b);
+        p.nk = kv_rows(a, p.b);
+        p.u0 = 0;
+        p.u1 = pl.units;
+        A::run(a, pl, smem, p, -1);
+        return;
+    }
+    const int p = (int)xcd_remap(blockIdx.x - pl.full, pl.shared);
+    ByLen<A::TR, A::KB> first64{};
+    const Share sh = shares(a, pl, first64, lane);
+    const unsigned end = sh.begin(p + 1);
+    for (unsigned u = sh.begin(p); u < end;) {
+        const Part t = part_at(a, pl, first64, u, end, lane);
+        u += t.u1 - t.u0;
+        A::run(a, pl, smem, t, t.u0 == 0 && t.u1 == t.n ? -1 : p + t.place);
+    }
+}
+
+// Joins the pieces of the shared tiles, in the order of their keys: HD/2 lanes a row, four columns of each map a lane.
+// PG groups of lanes take a row's pieces in turn (as many as a workgroup has beside few rows) and are merged in LDS.
+template <typename T, int HD, int TR, int KB, int PG>
+__global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs a, const DiffPlan pl) {
+    constexpr int LR = HD / 2, RPW = 256 / LR / PG, GROUPS = TR / RPW;   // rows of a workgroup; workgroups of a tile
+    __shared__ float4 part[PG > 1 ? 2 * 256 : 1];
+    __shared__ float4 stat[PG > 1 ? 256 / LR : 1];
+    const int lane = threadIdx.x & (LR - 1), team = (int)threadIdx.x / LR, rr = team % RPW, pg = team / RPW;
+    const int ts = (int)(blockIdx.x / GROUPS), r0 = (int)(blockIdx.x % GROUPS) * RPW, r = r0 + rr;
+    const int t = pl.full + ts, bg = t / pl.ntile, nkv = (int)a.nkv;
+    const int b = bg / nkv, g = bg - b * nkv, G = (int)(a.nh / a.nkv);
+    const int tile = tile_order(a, pl.ntile, t - bg * pl.ntile);
+    const int nq = q_rows(a, b);
+    if ((tile * TR + r0) / G >= nq) return;   // the whole workgroup
+    ByLen<TR, KB> x{};
+    const int wl = threadIdx.x & 63;
+    const Share sh = shares(a, pl, x, wl);
+    unsigned first = (unsigned)ts * pl.units, n = pl.units;
+    if (pl.by_len) {
+        unsigned before = 0;
+        while (x.b0 + 64 <= b) {
+            before += x.all();
+            x.look(a, x.b0 + 64, wl);
+        }
+        const int i = b - x.b0, heads = __builtin_amdgcn_readlane(x.tiles, i);
+        n = __builtin_amdgcn_readlane(x.n, i);
+        first = before + __builtin_amdgcn_readlane(x.upto - x.own, i) + (unsigned)(g * heads + tile_order(a, heads, tile)) * n;
+    }
+    const int p0 = (int)sh.holder(first), p1 = (int)sh.holder(first + n - 1);
+    if (p0 == p1) return;   // in one piece: written already
+    const RowOf ro = row_of(tile * TR + r, G);
+    const bool in = ro.qi < nq;
+    const int h = g * G + (in ? ro.hg : 0);
+    float m[2] = {-1e30f, -1e30f}, l[2] = {0.0f, 0.0f};
+    float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+    // one more part: the larger reference, what was before scaled to it
+    auto add = [&](int j, float mp, float lp, float4 v) {
+        const float mn = fmaxf(m[j], mp);
+        const float f = __builtin_amdgcn_exp2f(m[j] - mn), w = __builtin_amdgcn_exp2f(mp - mn);
+        m[j] = mn;
+        l[j] = l[j] * f + lp * w;
+        o[j] = make_float4(o[j].x * f + v.x * w, o[j].y * f + v.y * w, o[j].z * f + v.z * w, o[j].w * f + v.w * w);
+    };
+    if (in)
+#pragma unroll 2
+        for (int p = p0 + pg; p <= p1; p += PG) {
+            const long long row = (long long)(p + ts) * TR + r;
+            const float4 st = pl.st[row];
+            const float4 *v = (const float4 *)(pl.o + row * (4 * HD)) + lane;
+            const float4 v0 = v[0], v1 = v[HD / 2];
+            add(0, st.x, st.y, v0);
+            add(1, st.z, st.w, v1);
+        }
+    if constexpr (PG > 1) {
+        part[threadIdx.x] = o[0];
+        part[256 + threadIdx.x] = o[1];
+        if (lane == 0) stat[team] = make_float4(m[0], l[0], m[1], l[1]);
+        __syncthreads();
+        if (pg > 0) return;
+#pragma unroll
+        for (int k = 1; k < PG; ++k) {
+            const float4 st = stat[k * RPW + rr];
+            add(0, st.x, st.y, part[k * RPW * LR + threadIdx.x]);
+            add(1, st.z, st.w, part[256 + k * RPW * LR + threadIdx.x]);
         }
     }
     auto row_sum = [&](float v) {
@@ -628,15 +960,12 @@ __global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs 
     const float *lv = a.lam + (a.lam_heads > 1 ? (long long)h * 4 * HD : 0) + 2 * lane;
     const float d1 = row_sum(lv[0] * lv[HD] + lv[1] * lv[HD + 1]), d2 = row_sum(lv[2 * HD] * lv[3 * HD] + lv[2 * HD + 1] * lv[3 * HD + 1]);
     const float lam = expf(d1) - expf(d2) + a.lambda_init;
-    const float r0 = l[0] > 0.0f ? 1.0f / l[0] : 0.0f, r1 = l[1] > 0.0f ? lam / l[1] : 0.0f;
-    float y[4], ss = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        y[e] = o[0][e] * r0 - o[1][e] * r1;
-        ss += y[e] * y[e];
-    }
+    const float i0 = l[0] > 0.0f ? 1.0f / l[0] : 0.0f, i1 = l[1] > 0.0f ? lam / l[1] : 0.0f;
+    float y[4] = {o[0].x * i0 - o[1].x * i1, o[0].y * i0 - o[1].y * i1, o[0].z * i0 - o[1].z * i1, o[0].w * i0 - o[1].w * i1};
+    const float ss = row_sum((y[0] * y[0] + y[1] * y[1]) + (y[2] * y[2] + y[3] * y[3]));
+    if (!in) return;
     if (a.norm_w) {
-        const float f = (1.0f - a.lambda_init) / sqrtf(row_sum(ss) / (float)(2 * HD) + a.eps);
+        const float f = (1.0f - a.lambda_init) / sqrtf(ss / (float)(2 * HD) + a.eps);
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = y[e] * f * a.norm_w[4 * lane + e];
     }
@@ -650,14 +979,13 @@ bool chunked(const DiffAttnArgs &a) {
            ((a.ldq | a.ldk | a.ldv | a.ldo) & 7) == 0 && ((a.bsq | a.bsk | a.bsv | a.bso) & 7) == 0;
 }
 
-template <typename T, int HD, int RW, int KW>
+template <typename T, int HD, typename A>
 int launch_plan(const DiffAttnArgs &a, const DiffPlan &pl, hipStream_t st) {
-    TSN_LAUNCH((diff_attn_kernel<T, HD, RW, KW>), dim3((unsigned)(pl.full + pl.shared)), dim3(256), 0, st, a, pl);
+    TSN_LAUNCH((diff_attn_kernel<T, HD, A>), dim3((unsigned)(pl.full + pl.shared)), dim3(256), 0, st, a, pl);
     TSN_HIP_CHECK(hipGetLastError());
     if (pl.shared > 0) {
-        const long long rows = (long long)(pl.tiles - pl.full) * 32 * RW;
-        constexpr int RPW = 512 / HD;
-        TSN_LAUNCH((diff_attn_join_kernel<T, HD>), dim3((unsigned)((rows + RPW - 1) / RPW)), dim3(256), 0, st, a, pl, 32 * RW);
+        constexpr int PG = A::TR == 16 ? 8 : 1, GROUPS = A::TR * PG * HD / 512;
+        TSN_LAUNCH((diff_attn_join_kernel<T, HD, A::TR, A::KB, PG>), dim3((unsigned)(pl.tiles - pl.full) * GROUPS), dim3(256), 0, st, a, pl);
         TSN_HIP_CHECK(hipGetLastError());
     }
     return TSN_OK;
@@ -671,40 +999,70 @@ int launch_any(const DiffAttnArgs &a, hipStream_t st) {
     return TSN_OK;
 }
 
-// rows of a tile / 32, and what of the tiles is shared out
+// the rows of a tile, and what of the tiles is shared out
 struct DiffChoice {
-    int rw;
+    int rows, hd;
     DiffPlan pl;
-    size_t bytes() const {
-        return pl.shared ? (size_t)(pl.tiles - pl.full + pl.shared) * 32 * rw * (4 * hd + 4) * sizeof(float) : 0;
-    }
-    int hd;
+    size_t pieces() const { return pl.shared ? (size_t)(pl.tiles - pl.full + pl.shared) : 0; }
+    size_t bytes() const { return pieces() * rows * (4 * hd + 4) * sizeof(float); }
 };
 
+// The plan of the least estimated time (us, fitted to sweeps of 64 to 12289 rows and caches of 128 to 65536 keys; hd 32
+// takes 0.55 of hd 64's time a unit). 256 CUs hold two workgroups each.
+//  * wide tiles, a workgroup each: a unit takes 1.95 alone on a CU, 3.3 beside another
+//  * few-row tiles, a workgroup each: 0.95, 1.35
+//  * shared out: the same over 512 workgroups, and a second launch, and the pieces' way to memory and back
+// Measured, two samples of 8 heads, hd 64, full rows: 397 rows 11.7 few, 20.2 wide; 1101 rows 40.2, 39.7; 4096 rows 328,
+// 212. One row over 4099 keys, 8 heads: 33.7 a workgroup each, 12.2 shared; 64 sequences of 8192 keys: 200, 207.
 DiffChoice choose(const DiffAttnArgs &a) {
-    const long long rows = (long long)a.Sq * (a.nh / a.nkv);
+    const long long rows = (long long)a.Sq * (a.nh / a.nkv), heads = (long long)a.nkv * a.B;
+    const double h = a.hd == 64 ? 1.0 : 0.55;
+    const double stream = (double)heads * a.Sk * 8 * a.hd / 5.5e6;   // K and V from memory
+    const double seen = a.causal && a.Sq > a.Sk / 2 ? 0.55 : 1.0;    // of the keys, by many rows
+    const double ragged = a.kv_len ? 0.8 : 1.0;                      // a guess: a longer tile makes no one wait when shared
     DiffChoice best{};
-    double least = 1e30;
-    for (int rw : {4, 2, 1}) {
+    double least = 1e300;
+    for (int tr : {128, 16}) {
         DiffChoice c{};
-        c.rw = rw;
+        c.rows = tr;
         c.hd = (int)a.hd;
         DiffPlan &p = c.pl;
-        const int kb = rw == 1 ? 128 : 64;
-        p.ntile = (int)((rows + 32 * rw - 1) / (32 * rw));
-        const long long tiles = (long long)p.ntile * a.nkv * a.B;
-        if (tiles >= (1LL << 31)) continue;
-        p.tiles = (int)tiles;
+        const int kb = tr == 16 ? 128 : 64;
+        p.ntile = (int)((rows + tr - 1) / tr);
+        p.tiles = (int)(p.ntile * heads);
         p.units = (int)((a.Sk + kb - 1) / kb);
-        const char *e = getenv("DA_PLAN");   // rw,full,shared
-        int er = 4, ef = -1, es = 0;
-        if (e) sscanf(e, "%d,%d,%d", &er, &ef, &es);
-        if (er != rw) continue;
-        p.full = ef < 0 ? p.tiles : ef < p.tiles ? ef : p.tiles;
-        p.shared = p.full < p.tiles ? es : 0;
-        if (p.shared > (long long)(p.tiles - p.full) * p.units) p.shared = (p.tiles - p.full) * p.units;
-        best = c;
-        (void)least;
+        const double n = p.units, alone = (tr == 16 ? 0.95 : 1.95) * h, pair = (tr == 16 ? 1.35 : 3.3) * h;
+        auto keep = [&](double us, int full, int shared) {
+            if (us >= least) return;
+            DiffChoice d = c;
+            d.pl.full = full;
+            d.pl.shared = shared;
+            d.pl.by_len = full == 0 && (a.q_len || a.kv_len);
+            if (d.bytes() > ((size_t)256 << 20)) return;
+            best = d;
+            least = us;
+        };
+        double us;
+        if (tr == 16) {
+            const double r = p.tiles / 512.0, rounds = r <= 1 ? 1 : 0.5 * (r + ceil(r));
+            us = 3 + std::max(rounds * (n * (p.tiles <= 256 ? alone : pair) * (r > 1 ? seen : 1) + 3), stream);
+        } else {
+            const int t = (p.tiles + 255) / 256;
+            us = 7 + std::max(n * (t / 2 * pair + t % 2 * alone) * (t > 1 ? seen : 1), stream);
+        }
+        keep(us, p.tiles, 0);
+        if ((long long)p.tiles * p.units >= (1LL << 31) || p.tiles >= (1 << 24)) continue;
+        for (int wgs : {512, 256}) {   // all tiles, or those behind the last full round, shared out
+            for (int full : {0, p.tiles / 512 * 512}) {
+                const int rest = p.tiles - full;
+                const long long units = (long long)rest * p.units;
+                if (rest == 0 || (full == 0 && p.tiles > 512) || (full > 0 && tr == 16)) continue;
+                const int shared = (int)std::min<long long>(wgs, units);
+                const double part = ceil((double)units / shared) * (wgs == 512 ? pair : alone) * ragged;
+                const double pieces = 2.0 * std::min<double>(shared + rest, units) * std::min<double>(tr, rows) * 16.25 * a.hd / 6e6;
+                keep(9 + n * (full / 512) * pair + std::max(part, stream * ragged) + pieces + (tr == 16 ? rest / 100.0 : 0.0), full, shared);
+            }
+        }
     }
     return best;
 }
@@ -767,12 +1125,10 @@ int launch_diff_attention(const DiffAttnArgs &a, void *ws, size_t ws_bytes, hipS
         if (!chunked(a)) return a.hd == 64 ? launch_any<T, 64>(a, st) : launch_any<T, 32>(a, st);
         DiffChoice c = choose(a);
         TSN_REQUIRE(c.bytes() <= ws_bytes && (c.bytes() == 0 || ((uintptr_t)ws & 15) == 0), "diff_attention: workspace");
-        const size_t pieces = (size_t)(c.pl.tiles - c.pl.full + c.pl.shared) * 32 * c.rw;
         c.pl.st = (float4 *)ws;
-        c.pl.o = (float *)ws + 4 * pieces;
-        if (a.hd == 64)
-            return c.rw == 4 ? launch_plan<T, 64, 4, 1>(a, c.pl, st) : c.rw == 2 ? launch_plan<T, 64, 2, 2>(a, c.pl, st) : launch_plan<T, 64, 1, 4>(a, c.pl, st);
-        return c.rw == 4 ? launch_plan<T, 32, 4, 1>(a, c.pl, st) : c.rw == 2 ? launch_plan<T, 32, 2, 2>(a, c.pl, st) : launch_plan<T, 32, 1, 4>(a, c.pl, st);
+        c.pl.o = (float *)ws + 4 * c.pieces() * c.rows;
+        if (a.hd == 64) return c.rows == 128 ? launch_plan<T, 64, Wide<T, 64>>(a, c.pl, st) : launch_plan<T, 64, Few<T, 64>>(a, c.pl, st);
+        return c.rows == 128 ? launch_plan<T, 32, Wide<T, 32>>(a, c.pl, st) : launch_plan<T, 32, Few<T, 32>>(a, c.pl, st);
     };
     return a.dt == DT_F16 ? typed(half_t()) : typed(bf16_t());
 }
