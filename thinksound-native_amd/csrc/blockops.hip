@@ -4,6 +4,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.h"
 
@@ -13,6 +14,11 @@
 namespace tsn {
 
 namespace {
+
+// Whether a launch's traffic goes past the 256 MB last-level cache whatever it does: then loads and stores that leave
+// the caches alone are faster (rotary positions, f16, 269 MB: 47.2 -> 43.6 us, 202 MB: 37.4 -> 33.4), below that a result
+// may be there for what reads it next (134 MB: 22.2 -> 23.2).
+inline bool passes_caches(size_t bytes) { return bytes >= ((size_t)192 << 20); }
 
 /* ---------------- rotary positions over several axes ---------------- */
 
@@ -78,14 +84,19 @@ __global__ __launch_bounds__(256) void rope_axes_any_kernel(const RopeKernelArgs
 struct RopeChunks {
     unsigned rb, per_head, per_row, head_magic, row_magic;
 };
-template <typename T, bool HALF>
+template <typename T, bool HALF, bool ONCE>
 __global__ __launch_bounds__(256) void rope_axes_kernel(const RopeKernelArgs a, const RopeChunks c) {
-    constexpr int VE = 16 / sizeof(T), UN = HALF ? 4 : 8;   // elements of a chunk; items in flight a thread
+    constexpr int VE = 16 / sizeof(T), UN = 4;   // elements of a chunk; items in flight a thread
     typedef T vec __attribute__((ext_vector_type(VE)));
     extern __shared__ float2 table[];   // [row of the workgroup][pair]
     const unsigned np = a.hd / 2, r0 = blockIdx.x * c.rb, rows = min(c.rb, a.rows - r0), items = rows * c.per_row;
     const T *x = (const T *)a.x + (long long)r0 * a.ldx;
     T *y = (T *)a.y + (long long)r0 * a.ldy;
+    auto load = [](const T *p) { return ONCE ? __builtin_nontemporal_load((const vec *)p) : *(const vec *)p; };
+    auto store = [](T *p, vec v) {
+        if constexpr (ONCE) __builtin_nontemporal_store(v, (vec *)p);
+        else *(vec *)p = v;
+    };
     auto place = [&](unsigned i, unsigned &r, unsigned &h, unsigned &p, unsigned &e0, unsigned &e1) {   // item i: row, head, first pair, chunks
         r = __umulhi(i, c.row_magic);
         const unsigned in_row = i - r * c.per_row;
@@ -124,8 +135,8 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(const RopeKernelArgs a, 
             unsigned r, h, p, e0, e1;
             place(i, r, h, p, e0, e1);
             const T *row = x + (unsigned long long)r * a.ldx + h * a.hd;
-            v0[u] = *(const vec *)(row + e0);
-            if constexpr (HALF) v1[u] = *(const vec *)(row + e1);
+            v0[u] = load(row + e0);
+            if constexpr (HALF) v1[u] = load(row + e1);
         }
         if (i0 == 0) fill();
 #pragma unroll
@@ -146,10 +157,10 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(const RopeKernelArgs a, 
                         w0[e] = (T)(f0 * cs.x - f1 * cs.y);
                         w1[e] = (T)(f0 * cs.y + f1 * cs.x);
                     }
-                    *(vec *)(row + e0) = w0;
-                    *(vec *)(row + e1) = w1;
+                    store(row + e0, w0);
+                    store(row + e1, w1);
                 } else {
-                    *(vec *)(row + e0) = v0[u];
+                    store(row + e0, v0[u]);
                 }
             } else {
                 vec w = v0[u];
@@ -161,7 +172,7 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(const RopeKernelArgs a, 
                     w[e] = (T)(f0 * cs.x - f1 * cs.y);
                     w[e + 1] = (T)(f0 * cs.y + f1 * cs.x);
                 }
-                *(vec *)(row + e0) = w;
+                store(row + e0, w);
             }
         }
     }
@@ -256,7 +267,7 @@ __global__ __launch_bounds__(256) void gate_norm_any_kernel(const GateNormArgs a
 // one read and one write. A wave (a group of W) takes `per` rows one after the other and keeps what they share:
 // y = n(x_out) * A + B with A = pre_w (1 + scale), B = pre_b (1 + scale) + shift, and z's G = f_scale gate post_w, D =
 // f_scale gate post_b, made anew where a row of mod begins.
-template <typename TX, typename TF, int W, int NC>
+template <typename TX, typename TF, int W, int NC, bool ONCE>
 __global__ __launch_bounds__(W > 1 ? 64 * W : 256, 2) void gate_norm_kernel(const GateNormArgs a, unsigned per) {
     constexpr int GROUPS = W > 1 ? 1 : 4;   // row groups of a workgroup
     __shared__ float red_all[GROUPS][W];
@@ -346,7 +357,7 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256, 2) void gate_norm_kernel(cons
         for (int c = 0; c < NC; ++c) {
             const unsigned k = c * 64 * W + first;
             x[c] += f[c] * inv * G[c] + D[c];
-            if (k < chunks) store8((TX *)a.x_out + (unsigned long long)r * a.ldo + 8 * k, x[c]);
+            if (k < chunks) store8((TX *)a.x_out + (unsigned long long)r * a.ldo + 8 * k, x[c], std::integral_constant<bool, ONCE>());
             else x[c] = floatx8{};
         }
         if (!a.y) continue;
@@ -357,9 +368,9 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256, 2) void gate_norm_kernel(cons
             if (k >= chunks) break;
             const floatx8 y = x[c] * pinv * A[c] + B[c];
             const unsigned long long at = (unsigned long long)r * a.ldy + 8 * k;
-            if (a.ydt == DT_F32) store8((float *)a.y + at, y);
-            else if (a.ydt == DT_F16) store8((half_t *)a.y + at, y);
-            else store8((bf16_t *)a.y + at, y);
+            if (a.ydt == DT_F32) store8((float *)a.y + at, y, std::integral_constant<bool, ONCE>());
+            else if (a.ydt == DT_F16) store8((half_t *)a.y + at, y, std::integral_constant<bool, ONCE>());
+            else store8((bf16_t *)a.y + at, y, std::integral_constant<bool, ONCE>());
         }
     }
 }
@@ -372,7 +383,11 @@ int launch_gate_norm_rows(const GateNormArgs &a, hipStream_t st) {
     const unsigned waves = (unsigned)(((unsigned long long)a.rows * W + 2047) / 2048);
     const unsigned per = a.mod_rows == 1 ? 1 : std::min(waves, 32u);
     const unsigned groups = (a.rows + per - 1) / per;
-    TSN_LAUNCH((gate_norm_kernel<TX, TF, W, NC>), dim3((groups + GROUPS - 1) / GROUPS), dim3(W > 1 ? 64 * W : 256), 0, st, a, per);
+    const dim3 grid((groups + GROUPS - 1) / GROUPS), block(W > 1 ? 64 * W : 256);
+    if (passes_caches((size_t)a.rows * a.H * (2 * sizeof(TX) + sizeof(TF) + (a.y ? elem_bytes(a.ydt) : 0))))
+        TSN_LAUNCH((gate_norm_kernel<TX, TF, W, NC, true>), grid, block, 0, st, a, per);
+    else
+        TSN_LAUNCH((gate_norm_kernel<TX, TF, W, NC, false>), grid, block, 0, st, a, per);
     TSN_HIP_CHECK(hipGetLastError());
     return TSN_OK;
 }
@@ -444,7 +459,7 @@ int launch_rope_axes(const RopeAxesArgs &c, hipStream_t st) {
         RopeChunks k{};
         k.per_head = c.half_split ? (a.total / 2 + (c.hd - a.total)) / ve : c.hd / ve;
         k.per_row = c.nh * k.per_head;
-        const unsigned un = c.half_split ? 4 : 8;
+        const unsigned un = 4;
         // rows that give a workgroup's threads `un` items each, but no more than leave every CU eight workgroups
         const unsigned long long fill = c.rows / 2048 + 1;
         k.rb = (unsigned)std::max<unsigned long long>(1, std::min<unsigned long long>({256 * un / k.per_row, fill, 16384 / c.hd}));
@@ -457,13 +472,18 @@ int launch_rope_axes(const RopeAxesArgs &c, hipStream_t st) {
         if (whole) {
             const dim3 grid((c.rows + k.rb - 1) / k.rb);
             const size_t lds = (size_t)k.rb * (c.hd / 2) * sizeof(float2);
-#define ROPE(T)                                                                                     \
-    if (c.half_split) TSN_LAUNCH((rope_axes_kernel<T, true>), grid, dim3(256), lds, st, a, k);      \
-    else TSN_LAUNCH((rope_axes_kernel<T, false>), grid, dim3(256), lds, st, a, k)
+            const bool once = passes_caches((size_t)2 * c.rows * c.nh * c.hd * elem_bytes(c.dt));
+#define ROPE_AS(T, HALF)                                                                                \
+    if (once) TSN_LAUNCH((rope_axes_kernel<T, HALF, true>), grid, dim3(256), lds, st, a, k);            \
+    else TSN_LAUNCH((rope_axes_kernel<T, HALF, false>), grid, dim3(256), lds, st, a, k)
+#define ROPE(T)                                   \
+    if (c.half_split) { ROPE_AS(T, true); }       \
+    else { ROPE_AS(T, false); }
             if (c.dt == DT_F32) { ROPE(float); }
             else if (c.dt == DT_F16) { ROPE(half_t); }
             else { ROPE(bf16_t); }
 #undef ROPE
+#undef ROPE_AS
             TSN_HIP_CHECK(hipGetLastError());
             return TSN_OK;
         }

@@ -29,9 +29,11 @@ template <typename T> struct Eight;
 template <> struct Eight<float> { typedef floatx8 type; };
 template <> struct Eight<half_t> { typedef half8 type; };
 template <> struct Eight<bf16_t> { typedef bf16x8_e type; };
-template <typename T>
-__device__ __forceinline__ void store8(T *p, const floatx8 &v) {
-    *(typename Eight<T>::type *)p = __builtin_convertvector(v, typename Eight<T>::type);
+template <typename T, typename ONCE>
+__device__ __forceinline__ void store8(T *p, const floatx8 &v, ONCE) {   // true_type: past the caches
+    const auto w = __builtin_convertvector(v, typename Eight<T>::type);
+    if constexpr (ONCE::value) __builtin_nontemporal_store(w, (typename Eight<T>::type *)p);
+    else *(typename Eight<T>::type *)p = w;
 }
 
 // rows of `width` bytes, `ld` bytes apart, in samples `bs` bytes apart
