@@ -141,6 +141,31 @@ def test_rope_axes(tsn, rt, dt, rows, nh, hd, dims, half, inverse, ldx, ldy, col
         b.free()
 
 
+def spread(n, r):
+    """rows of a large array that are looked at: both ends and some between"""
+    return np.unique(np.concatenate([np.arange(40), r.integers(0, n, 400), np.arange(n - 40, n)]))
+
+
+@pytest.mark.parametrize("dt,half", [(F32, False), (F16, True), (F16, False), (BF16, True)])
+def test_rope_axes_large(tsn, rt, dt, half):
+    """traffic past the last-level cache (over 192 MiB), an odd number of rows"""
+    r = rng(12)
+    nh, hd, dims, bases = 32, 64, (16, 16, 32), (1e4, 1e2, 1e2)
+    rows = (13 if dt == F32 else 26) * 1000 + 1
+    some = enc(r.standard_normal((997, nh * hd)), dt)
+    x = some[np.arange(rows) % 997]
+    pos = r.integers(0, 5000, (rows, 3)).astype(np.int32)
+    xb, pb, yb = rt.array(x), rt.array(pos), rt.array(np.full(x.shape, SENTINEL[dt], NP[dt]))
+    rt.rope_axes(tsn.rope_axes_spec(dt, rows, nh, hd, dims, bases, half_split=half), xb, pb, yb)
+    rt.sync()
+    at = spread(rows, r)
+    got, xf = dec(yb.numpy()[at], dt).reshape(len(at), nh, hd), dec(x[at], dt).reshape(len(at), nh, hd)
+    want = rope_ref(xf, pos[at], dims, bases, (1.0,) * 3, half, False)
+    check(got, want, rope_tol(xf, dt, want, dims, half))
+    for b in (xb, pb, yb):
+        b.free()
+
+
 def test_rope_axes_one_axis_is_rope_pairs(tsn, rt):
     """n_axes = 1 over the whole head is tsn_rope_pairs; its angle is rounded to f32 at up to 171 rad (2^-17 of a
     radian), its product with the frequency and powf add as much again twice: 2^-15 of |x0| + |x1| between the two"""
@@ -275,6 +300,30 @@ def test_gate_add_norm(tsn, rt, rows, H, xdt, fdt, ydt, post, pre, mod_rows, chu
         b.free()
 
 
+@pytest.mark.parametrize("H,xdt,fdt,ydt,mod_rows", [(2048, BF16, BF16, BF16, 1), (1000, F32, F16, F16, 397), (504, F16, F32, BF16, 5000)])
+def test_gate_add_norm_large(tsn, rt, H, xdt, fdt, ydt, mod_rows):
+    """traffic past the last-level cache (over 192 MiB), rows that several waves take in turn"""
+    r = rng(H)
+    size = lambda dt: 4 if dt == F32 else 2  # noqa: E731
+    rows = (202 << 20) // (H * (2 * size(xdt) + size(fdt) + size(ydt))) + 1
+    x, f = (enc(r.standard_normal((991, H)), dt)[np.arange(rows) % 991] for dt in (xdt, fdt))
+    mod = (0.3 * r.standard_normal((-(-rows // mod_rows), 3 * H))).astype(np.float32)
+    w = (1.0 + 0.1 * r.standard_normal(H)).astype(np.float32)
+    c = dict(post=2, pre=1, x_scale=0.9, f_scale=1.1, mod_rows=mod_rows, gate=2, shift=0, scale=1, post_eps=1e-5, pre_eps=1e-6)
+    xb, fb, mb, wb = rt.array(x), rt.array(f), rt.array(mod), rt.array(w)
+    ob, yb = rt.array(np.full(x.shape, SENTINEL[xdt], NP[xdt])), rt.array(np.full(x.shape, SENTINEL[ydt], NP[ydt]))
+    rt.gate_add_norm(tsn.gate_norm_spec(rows, H, xdt, fdt, ydt, chunks=3, **c), xb, fb, mb, ob, yb, post_w=wb, pre_w=wb)
+    rt.sync()
+    at = spread(rows, r)
+    c.update(mod_rows=1, **{k: np.float64(np.float32(c[k])) for k in ("post_eps", "pre_eps")})
+    ws = dict(post_w=w.astype(np.float64), pre_w=w.astype(np.float64))
+    xo, ex, y, ty = gate_norm_ref(dec(x[at], xdt), dec(f[at], fdt), mod[at // mod_rows], c, ws)
+    check(dec(ob.numpy()[at], xdt), xo, ex + U[xdt] * (np.abs(xo) + ex) + TINY[xdt], "x_out")
+    check(dec(yb.numpy()[at], ydt), y, ty + U[ydt] * (np.abs(y) + ty) + TINY[ydt], "y")
+    for b in (xb, fb, mb, wb, ob, yb):
+        b.free()
+
+
 def test_gate_add_norm_is_gate_add_then_adaln(tsn, rt):
     """without norm and weights on the block's side it is tsn_gate_add followed by tsn_adaln_ln"""
     r = rng(8)
@@ -293,18 +342,20 @@ def test_gate_add_norm_is_gate_add_then_adaln(tsn, rt):
 
 # ---------------------------------------------------------------- differential attention
 
-def attn_ref(q, k, v, lam, w, ql, kl, causal, scale, lambda_init, eps, nh, nkv, hd, dt):
-    """(out, bound, live) in f64; q [B][Sq][nh*2*hd] and so on are the values that the elements stand for"""
+def attn_ref(q, k, v, lam, w, ql, kl, causal, scale, lambda_init, eps, nh, nkv, hd, dt, heads=None):
+    """(out, bound, live) in f64; q [B][Sq][nh*2*hd] and so on are the values that the elements stand for. heads: those
+    that are computed, the others are not live"""
     B, Sq, _ = q.shape
     Sk = k.shape[1]
     out, tol, live = np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape, bool)
     for b in range(B):
         n, m = int(np.clip(ql[b], 0, Sq)), int(np.clip(kl[b], 0, Sk))
-        live[b, :n] = True
+        for h in range(nh) if heads is None else heads:
+            live[b, :n, 2 * h * hd:2 * (h + 1) * hd] = True
         if n == 0 or m == 0:
             continue
         seen = np.arange(m)[None] <= (np.arange(n)[:, None] + (m - n) if causal else m)
-        for h in range(nh):
+        for h in range(nh) if heads is None else heads:
             g = h * nkv // nh
             L = lam[h if lam.shape[0] > 1 else 0]
             lm = np.exp(L[0] @ L[1]) - np.exp(L[2] @ L[3]) + lambda_init
@@ -336,7 +387,7 @@ def attn_ref(q, k, v, lam, w, ql, kl, causal, scale, lambda_init, eps, nh, nkv, 
 
 
 def attn_case(tsn, rt, dt, B, Sq, Sk, nh, nkv, hd, causal=False, ql=None, kl=None, lam_heads=1, norm=True, scale=None,
-              lambda_init=0.5, pad=(0, 0, 0, 0), make=None, seed=0, junk=None, col=0):
+              lambda_init=0.5, pad=(0, 0, 0, 0), make=None, seed=0, junk=None, col=0, heads=None):
     """Runs one call and checks every element, the rows behind q_len and the columns around the heads. pad: elements
     behind the packed row of q, k, v, out; col: first column of each."""
     r = rng(seed + 31 * Sq + 7 * Sk + hd)
@@ -364,11 +415,13 @@ def attn_case(tsn, rt, dt, B, Sq, Sk, nh, nkv, hd, causal=False, ql=None, kl=Non
     ql2, kl2 = ([Sq] * B if ql is None else ql), ([Sk] * B if kl is None else kl)
     want, tol, live = attn_ref(*(dec(t, dt) for t in (q, k, v)), lam.astype(np.float64), None if w is None else w.astype(np.float64), ql2, kl2,
                                causal, np.float64(np.float32(hd ** -0.5 if scale is None else scale)), np.float64(np.float32(lambda_init)),
-                               np.float64(np.float32(1e-5)), nh, nkv, hd, dt)
+                               np.float64(np.float32(1e-5)), nh, nkv, hd, dt, heads)
     res = first[:, col:col + wq].reshape(B, Sq, wq)
     got = dec(res, dt)
     check(got[live], want[live], tol[live])
-    assert (res[~live] == SENTINEL[dt]).all(), "rows behind q_len were written"
+    behind = np.arange(Sq)[None, :] >= np.maximum(np.asarray(ql2), 0)[:, None]
+    assert (res[behind] == SENTINEL[dt]).all(), "rows behind q_len were written"
+    assert heads is not None or (live != behind[:, :, None]).all()
     assert (np.delete(first, np.s_[col:col + wq], 1) == SENTINEL[dt]).all(), "columns around the heads were written"
     rt.diff_attention(spec, *args)
     rt.sync()
@@ -396,6 +449,34 @@ def test_diff_attention(tsn, rt, dt, hd, B, Sq, Sk, nh, nkv, causal):
         # the rounding of the result and those of the probabilities are independent: u/sqrt(3) each at most (the
         # two maps' add as the squares of their shares of the difference); 2u is over twice their joint size
         assert rel_l2(got, want) <= 2 * U[dt]
+
+
+# sizes at which the work is cut in each way, and the cuts fall inside tiles
+CUTS = [
+    # B Sq Sk nh nkv causal kl heads
+    (130, 1, 4000, 2, 1, True, "ragged", None),        # one row of more than 64 samples: shared out by the lengths
+    (70, 3, 1500, 2, 1, False, "some empty", None),
+    (1, 1, 70000, 2, 1, False, None, None),            # one row over a long cache
+    (2, 40, 6000, 4, 1, True, "ragged", None),         # several tiles of few rows
+    (1, 1000, 8192, 4, 4, True, None, (0, 3)),         # wide tiles shared out
+    (2, 600, 9000, 2, 2, False, "ragged", None),
+    (1, 1300, 3000, 50, 50, False, None, (0, 24, 46, 49)),   # the tiles behind the last full round shared out
+    (3, 1000, 2500, 24, 24, False, "ragged", (0, 11, 23)),
+    (1, 2500, 2500, 8, 8, True, None, (2, 7)),         # causal tiles, heads round the XCDs
+    (4, 500, 500, 6, 2, True, "ragged", (0, 5)),
+]
+
+
+@pytest.mark.parametrize("dt,hd", [(F16, 64), (BF16, 32)])
+@pytest.mark.parametrize("B,Sq,Sk,nh,nkv,causal,kl,heads", CUTS)
+def test_diff_attention_cuts(tsn, rt, dt, hd, B, Sq, Sk, nh, nkv, causal, kl, heads):
+    r = rng(B + Sq)
+    lens = None if kl is None else [int(t) for t in r.integers(Sk // 4, Sk + 1, B)]
+    ql = None
+    if kl == "some empty":
+        lens[3], lens[65], lens[69] = 0, 1, 0
+        ql = [int(t) for t in r.integers(0, Sq + 1, B)]
+    attn_case(tsn, rt, dt, B, Sq, Sk, nh, nkv, hd, causal, ql, lens, junk=None if kl is None else np.nan, heads=heads)
 
 
 @pytest.mark.parametrize("hd", [64, 32])

@@ -61,19 +61,20 @@ __device__ __forceinline__ void turn(double freq, int pos, float &cs, float &sn)
 // are taken once.
 __global__ __launch_bounds__(256) void rope_axes_any_kernel(const RopeKernelArgs a) {
     const unsigned np = a.hd / 2;
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (id >= (long long)a.rows * np) return;
-    const unsigned r = (unsigned)(id / np), p = (unsigned)(id - (long long)r * np);
-    unsigned axis, e0, e1;
-    pair_at(a, p, axis, e0, e1);
-    float cs, sn;
-    turn(a.freq[p], a.pos[(long long)(r % a.pos_rows) * a.n_axes + axis], cs, sn);
-    const long long xr = (long long)r * a.ldx, yr = (long long)r * a.ldy;
-    const bool turned = 2 * p < a.total;
-    for (unsigned h = 0; h < a.nh; ++h) {
-        const float v0 = load_elem(a.x, a.dt, xr + h * a.hd + e0), v1 = load_elem(a.x, a.dt, xr + h * a.hd + e1);
-        store_elem(a.y, a.dt, yr + h * a.hd + e0, turned ? v0 * cs - v1 * sn : v0);
-        store_elem(a.y, a.dt, yr + h * a.hd + e1, turned ? v0 * sn + v1 * cs : v1);
+    const long long n = (long long)a.rows * np;
+    for (long long id = (long long)blockIdx.x * 256 + threadIdx.x; id < n; id += (long long)gridDim.x * 256) {
+        const unsigned r = (unsigned)(id / np), p = (unsigned)(id - (long long)r * np);
+        unsigned axis, e0, e1;
+        pair_at(a, p, axis, e0, e1);
+        float cs, sn;
+        turn(a.freq[p], a.pos[(long long)(r % a.pos_rows) * a.n_axes + axis], cs, sn);
+        const long long xr = (long long)r * a.ldx, yr = (long long)r * a.ldy;
+        const bool turned = 2 * p < a.total;
+        for (unsigned h = 0; h < a.nh; ++h) {
+            const float v0 = load_elem(a.x, a.dt, xr + h * a.hd + e0), v1 = load_elem(a.x, a.dt, xr + h * a.hd + e1);
+            store_elem(a.y, a.dt, yr + h * a.hd + e0, turned ? v0 * cs - v1 * sn : v0);
+            store_elem(a.y, a.dt, yr + h * a.hd + e1, turned ? v0 * sn + v1 * cs : v1);
+        }
     }
 }
 
@@ -196,70 +197,72 @@ __device__ __forceinline__ float group_sum(float v, float *red) {
     return v;
 }
 
-// Any width, stride and alignment: one workgroup a row, the row (f, then x_out) in LDS as f32.
+// Any width, stride and alignment: a workgroup takes a row at a time, the row (f, then x_out) in LDS as f32.
 __global__ __launch_bounds__(256) void gate_norm_any_kernel(const GateNormArgs a) {
     extern __shared__ float row[];
     __shared__ float red[4];
-    const unsigned r = blockIdx.x, H = a.H;
+    const unsigned H = a.H;
     const int tid = threadIdx.x;
-    const long long xr = (long long)r * a.ldx, fr = (long long)r * a.ldf, orow = (long long)r * a.ldo, yr = (long long)r * a.ldy;
-    const float *mod = a.mod ? a.mod + (long long)(r / a.mod_rows) * a.chunks * H : nullptr;
     const float n = (float)H;
-    // a thread reads back only elements that it wrote itself
-    float s = 0.0f;
-    for (unsigned i = tid; i < H; i += 256) {
-        const float v = load_elem(a.f, a.fdt, fr + i);
-        row[i] = v;
-        s += a.post == NORM_LN ? v : v * v;
-    }
-    float mean = 0.0f, inv = 1.0f;
-    if (a.post != NORM_NONE) {
-        s = group_sum<4>(s, red);
-        if (a.post == NORM_LN) {
-            mean = s / n;
-            s = 0.0f;
-            for (unsigned i = tid; i < H; i += 256) {
-                const float d = row[i] - mean;
-                s += d * d;
-            }
-            s = group_sum<4>(s, red);
+    for (unsigned r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const long long xr = (long long)r * a.ldx, fr = (long long)r * a.ldf, orow = (long long)r * a.ldo, yr = (long long)r * a.ldy;
+        const float *mod = a.mod ? a.mod + (long long)(r / a.mod_rows) * a.chunks * H : nullptr;
+        // a thread reads back only elements that it wrote itself
+        float s = 0.0f;
+        for (unsigned i = tid; i < H; i += 256) {
+            const float v = load_elem(a.f, a.fdt, fr + i);
+            row[i] = v;
+            s += a.post == NORM_LN ? v : v * v;
         }
-        inv = 1.0f / sqrtf(s / n + a.post_eps);
-    }
-    s = 0.0f;
-    for (unsigned i = tid; i < H; i += 256) {
-        float z = (row[i] - mean) * inv;
-        if (a.post_w) z *= a.post_w[i];
-        if (a.post_b) z += a.post_b[i];
-        const float g = a.f_scale * (a.gate >= 0 ? mod[(long long)a.gate * H + i] : 1.0f);
-        const float v = a.x_scale * load_elem(a.x, a.xdt, xr + i) + g * z;
-        store_elem(a.x_out, a.xdt, orow + i, v);
-        row[i] = v;
-        s += a.pre == NORM_LN ? v : v * v;
-    }
-    if (!a.y) return;
-    mean = 0.0f;
-    inv = 1.0f;
-    if (a.pre != NORM_NONE) {
-        s = group_sum<4>(s, red);
-        if (a.pre == NORM_LN) {
-            mean = s / n;
-            s = 0.0f;
-            for (unsigned i = tid; i < H; i += 256) {
-                const float d = row[i] - mean;
-                s += d * d;
-            }
+        float mean = 0.0f, inv = 1.0f;
+        if (a.post != NORM_NONE) {
             s = group_sum<4>(s, red);
+            if (a.post == NORM_LN) {
+                mean = s / n;
+                s = 0.0f;
+                for (unsigned i = tid; i < H; i += 256) {
+                    const float d = row[i] - mean;
+                    s += d * d;
+                }
+                s = group_sum<4>(s, red);
+            }
+            inv = 1.0f / sqrtf(s / n + a.post_eps);
         }
-        inv = 1.0f / sqrtf(s / n + a.pre_eps);
-    }
-    for (unsigned i = tid; i < H; i += 256) {
-        float v = (row[i] - mean) * inv;
-        if (a.pre_w) v *= a.pre_w[i];
-        if (a.pre_b) v += a.pre_b[i];
-        if (a.scale >= 0) v *= 1.0f + mod[(long long)a.scale * H + i];
-        if (a.shift >= 0) v += mod[(long long)a.shift * H + i];
-        store_elem(a.y, a.ydt, yr + i, v);
+        s = 0.0f;
+        for (unsigned i = tid; i < H; i += 256) {
+            float z = (row[i] - mean) * inv;
+            if (a.post_w) z *= a.post_w[i];
+            if (a.post_b) z += a.post_b[i];
+            const float g = a.f_scale * (a.gate >= 0 ? mod[(long long)a.gate * H + i] : 1.0f);
+            const float v = a.x_scale * load_elem(a.x, a.xdt, xr + i) + g * z;
+            store_elem(a.x_out, a.xdt, orow + i, v);
+            row[i] = v;
+            s += a.pre == NORM_LN ? v : v * v;
+        }
+        if (!a.y) continue;
+        mean = 0.0f;
+        inv = 1.0f;
+        if (a.pre != NORM_NONE) {
+            s = group_sum<4>(s, red);
+            if (a.pre == NORM_LN) {
+                mean = s / n;
+                s = 0.0f;
+                for (unsigned i = tid; i < H; i += 256) {
+                    const float d = row[i] - mean;
+                    s += d * d;
+                }
+                s = group_sum<4>(s, red);
+            }
+            inv = 1.0f / sqrtf(s / n + a.pre_eps);
+        }
+        for (unsigned i = tid; i < H; i += 256) {
+            float v = (row[i] - mean) * inv;
+            if (a.pre_w) v *= a.pre_w[i];
+            if (a.pre_b) v += a.pre_b[i];
+            if (a.scale >= 0) v *= 1.0f + mod[(long long)a.scale * H + i];
+            if (a.shift >= 0) v += mod[(long long)a.shift * H + i];
+            store_elem(a.y, a.ydt, yr + i, v);
+        }
     }
 }
 
@@ -268,7 +271,7 @@ __global__ __launch_bounds__(256) void gate_norm_any_kernel(const GateNormArgs a
 // y = n(x_out) * A + B with A = pre_w (1 + scale), B = pre_b (1 + scale) + shift, and z's G = f_scale gate post_w, D =
 // f_scale gate post_b, made anew where a row of mod begins.
 template <typename TX, typename TF, int W, int NC, bool ONCE>
-__global__ __launch_bounds__(W > 1 ? 64 * W : 256, 2) void gate_norm_kernel(const GateNormArgs a, unsigned per) {
+__global__ __launch_bounds__(W > 1 ? 64 * W : 256, NC == 1 ? 4 : 2) void gate_norm_kernel(const GateNormArgs a, unsigned per) {
     constexpr int GROUPS = W > 1 ? 1 : 4;   // row groups of a workgroup
     __shared__ float red_all[GROUPS][W];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -378,11 +381,13 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256, 2) void gate_norm_kernel(cons
 template <typename TX, typename TF, int W, int NC>
 int launch_gate_norm_rows(const GateNormArgs &a, hipStream_t st) {
     constexpr unsigned GROUPS = W > 1 ? 1 : 4;
-    // Rows that share a row of mod in turn, so that the waves fill the device once (eight a CU): 6352 rows of 1024 take
-    // 22.2 us a row a wave, 16.6 us four rows a wave (4.7 TB/s). A row of mod of its own: a row a wave.
-    const unsigned waves = (unsigned)(((unsigned long long)a.rows * W + 2047) / 2048);
-    const unsigned per = a.mod_rows == 1 ? 1 : std::min(waves, 32u);
-    const unsigned groups = (a.rows + per - 1) / per;
+    // Rows that share a row of mod in turn, so that the waves fill the device once (16 or 8 a CU): 6352 rows of 1024 take
+    // 22.2 us a row a wave, 16.6 us four rows a wave, 15.8 us four rows two waves (4.9 TB/s). A row of mod of its own:
+    // a row a group, and many groups waiting for a place.
+    constexpr unsigned AT_ONCE = NC == 1 ? 4096 : 2048;
+    const unsigned waves = (unsigned)(((unsigned long long)a.rows * W + AT_ONCE - 1) / AT_ONCE);
+    const unsigned per = std::max(a.mod_rows == 1 ? 1u : std::min(waves, 32u), (a.rows >> 22) + 1);   // a launch has less than 2^32 threads
+    const unsigned groups = a.rows / per + (a.rows % per != 0);
     const dim3 grid((groups + GROUPS - 1) / GROUPS), block(W > 1 ? 64 * W : 256);
     if (passes_caches((size_t)a.rows * a.H * (2 * sizeof(TX) + sizeof(TF) + (a.y ? elem_bytes(a.ydt) : 0))))
         TSN_LAUNCH((gate_norm_kernel<TX, TF, W, NC, true>), grid, block, 0, st, a, per);
@@ -394,7 +399,7 @@ int launch_gate_norm_rows(const GateNormArgs &a, hipStream_t st) {
 template <typename TX, typename TF>
 int launch_gate_norm_typed(const GateNormArgs &a, hipStream_t st) {
     if (a.H <= 512) return launch_gate_norm_rows<TX, TF, 1, 1>(a, st);
-    if (a.H <= 1024) return launch_gate_norm_rows<TX, TF, 1, 2>(a, st);
+    if (a.H <= 1024) return launch_gate_norm_rows<TX, TF, 2, 1>(a, st);
     if (a.H <= 2048) return launch_gate_norm_rows<TX, TF, 2, 2>(a, st);
     if (a.H <= 4096) return launch_gate_norm_rows<TX, TF, 4, 2>(a, st);
     return launch_gate_norm_rows<TX, TF, 8, 2>(a, st);   // to 8192
@@ -421,8 +426,7 @@ int rope_axes_check(RopeAxesArgs &a) {
     }
     TSN_REQUIRE(total <= a.hd, "rope_axes: the axes turn more than hd elements");
     const unsigned long long n = (unsigned long long)a.nh * a.hd;
-    TSN_REQUIRE(n < (1ULL << 31) && (unsigned long long)a.rows * (a.hd / 2) < (1ULL << 31) * 128,
-                "rope_axes: sizes beyond the launch grid");
+    TSN_REQUIRE(n < (1ULL << 31), "rope_axes: rows of 2^31 elements or more");
     if (!a.ldx) a.ldx = (uint32_t)n;
     if (!a.ldy) a.ldy = (uint32_t)n;
     TSN_REQUIRE(a.ldx >= n && a.ldy >= n, "rope_axes: row stride below the row width");
@@ -463,12 +467,13 @@ int launch_rope_axes(const RopeAxesArgs &c, hipStream_t st) {
         // rows that give a workgroup's threads `un` items each, but no more than leave every CU eight workgroups
         const unsigned long long fill = c.rows / 2048 + 1;
         k.rb = (unsigned)std::max<unsigned long long>(1, std::min<unsigned long long>({256 * un / k.per_row, fill, 16384 / c.hd}));
+        k.rb = std::max(k.rb, c.rows >> 23);   // a launch has less than 2^32 threads
         // i / d = umulhi(i, magic) while i * d < 2^32
         auto magic = [](unsigned d) { return d == 1 ? 0u : (unsigned)((0x100000000ULL + d - 1) / d); };
         k.head_magic = magic(k.per_head);
         k.row_magic = magic(k.per_row);
         const unsigned long long most = (unsigned long long)k.rb * k.per_row;
-        whole = k.per_head > 1 && most * k.per_row < (1ULL << 32);
+        whole = k.per_head > 1 && most * k.per_row < (1ULL << 32) && k.rb <= 16384 / c.hd;
         if (whole) {
             const dim3 grid((c.rows + k.rb - 1) / k.rb);
             const size_t lds = (size_t)k.rb * (c.hd / 2) * sizeof(float2);
@@ -489,7 +494,7 @@ int launch_rope_axes(const RopeAxesArgs &c, hipStream_t st) {
         }
     }
     const unsigned long long n = (unsigned long long)c.rows * (c.hd / 2);
-    TSN_LAUNCH(rope_axes_any_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+    TSN_LAUNCH(rope_axes_any_kernel, dim3((unsigned)std::min<unsigned long long>((n + 255) / 256, 1 << 20)), dim3(256), 0, st, a);
     TSN_HIP_CHECK(hipGetLastError());
     return TSN_OK;
 }
@@ -499,7 +504,6 @@ int gate_add_norm_check(GateNormArgs &a) {
     TSN_REQUIRE(is_elem(a.xdt) && is_elem(a.fdt) && is_elem(a.ydt), "gate_add_norm: dtypes f32, f16 or bf16");
     TSN_REQUIRE(a.post >= NORM_NONE && a.post <= NORM_LN && a.pre >= NORM_NONE && a.pre <= NORM_LN, "gate_add_norm: norm kind");
     TSN_REQUIRE(a.rows > 0 && a.H > 0, "gate_add_norm: empty shape");
-    TSN_REQUIRE(a.rows < (1u << 31), "gate_add_norm: sizes beyond the launch grid");
     if (a.H > 16384) {
         set_error("gate_add_norm: H above 16384");
         return TSN_ERR_UNSUPPORTED;
@@ -548,7 +552,7 @@ int launch_gate_add_norm(const GateNormArgs &a, hipStream_t st) {
         if (a.xdt == DT_F32) return launch_gate_norm_f<float>(a, st);
         return a.xdt == DT_F16 ? launch_gate_norm_f<half_t>(a, st) : launch_gate_norm_f<bf16_t>(a, st);
     }
-    TSN_LAUNCH(gate_norm_any_kernel, dim3(a.rows), dim3(256), a.H * sizeof(float), st, a);
+    TSN_LAUNCH(gate_norm_any_kernel, dim3(std::min(a.rows, 1u << 20)), dim3(256), a.H * sizeof(float), st, a);
     TSN_HIP_CHECK(hipGetLastError());
     return TSN_OK;
 }

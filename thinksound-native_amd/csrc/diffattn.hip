@@ -43,67 +43,69 @@ __global__ __launch_bounds__(256) void diff_attn_any_kernel(const DiffAttnArgs a
     __shared__ float sq[4][2 * HD];
     __shared__ float sp[4][2][64];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const long long id = (long long)blockIdx.x * 4 + wave;
     const long long n_items = (long long)a.B * a.Sq * a.nh;
-    if (id >= n_items) return;   // no barrier below: a wave uses its own LDS
-    const int h = (int)(id % a.nh);
-    const long long br = id / a.nh;
-    const int b = (int)(br / a.Sq), r = (int)(br - (long long)b * a.Sq);
-    const int nq = q_rows(a, b), nk = kv_rows(a, b);
-    if (r >= nq) return;
-    const int g = h / (int)(a.nh / a.nkv);
-    int keys = nk;
-    if (a.causal) keys = min(nk, max(0, r + nk - nq + 1));
-    const T *q = (const T *)a.q + (long long)b * a.bsq + (long long)r * a.ldq + (long long)h * 2 * HD;
-    const T *k = (const T *)a.k + (long long)b * a.bsk + (long long)g * 2 * HD;
-    const T *v = (const T *)a.v + (long long)b * a.bsv + (long long)g * 2 * HD;
-    for (int i = lane; i < 2 * HD; i += 64) sq[wave][i] = (float)q[i] * a.scale * LOG2E;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[2][NV] = {};
-    for (int k0 = 0; k0 < keys; k0 += 64) {
-        const int n = min(64, keys - k0);
-        float s[2] = {-INFINITY, -INFINITY};
-        if (lane < n) {
-            const T *kr = k + (long long)(k0 + lane) * a.ldk;
+    for (long long id = (long long)blockIdx.x * 4 + wave; id < n_items; id += (long long)gridDim.x * 4) {   // no barrier: a wave uses its own LDS
+        const int h = (int)(id % a.nh);
+        const long long br = id / a.nh;
+        const int b = (int)(br / a.Sq), r = (int)(br - (long long)b * a.Sq);
+        const int nq = q_rows(a, b), nk = kv_rows(a, b);
+        if (r >= nq) continue;
+        const int g = h / (int)(a.nh / a.nkv);
+        int keys = nk;
+        if (a.causal) keys = min(nk, max(0, r + nk - nq + 1));
+        const T *q = (const T *)a.q + (long long)b * a.bsq + (long long)r * a.ldq + (long long)h * 2 * HD;
+        const T *k = (const T *)a.k + (long long)b * a.bsk + (long long)g * 2 * HD;
+        const T *v = (const T *)a.v + (long long)b * a.bsv + (long long)g * 2 * HD;
+        for (int i = lane; i < 2 * HD; i += 64) sq[wave][i] = (float)q[i] * a.scale * LOG2E;
+        __builtin_amdgcn_wave_barrier();   // a wave's LDS accesses are done in their order
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[2][NV] = {};
+        for (int k0 = 0; k0 < keys; k0 += 64) {
+            const int n = min(64, keys - k0);
+            float s[2] = {-INFINITY, -INFINITY};
+            if (lane < n) {
+                const T *kr = k + (long long)(k0 + lane) * a.ldk;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float d = 0.0f;
+                    for (int i = 0; i < HD; ++i) d += sq[wave][j * HD + i] * (float)kr[j * HD + i];
+                    s[j] = d;
+                }
+            }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                float d = 0.0f;
-                for (int i = 0; i < HD; ++i) d += sq[wave][j * HD + i] * (float)kr[j * HD + i];
-                s[j] = d;
+                const float mn = fmaxf(m[j], wave_max(s[j]));
+                const float al = exp2f(m[j] - mn), p = lane < n ? exp2f(s[j] - mn) : 0.0f;
+                m[j] = mn;
+                l[j] = l[j] * al + wave_sum(p);
+                for (int c = 0; c < NV; ++c) o[j][c] *= al;
+                sp[wave][j][lane] = p;
+            }
+            __builtin_amdgcn_wave_barrier();
+            for (int t = 0; t < n; ++t) {
+                const T *vr = v + (long long)(k0 + t) * a.ldv;
+#pragma unroll
+                for (int c = 0; c < NV; ++c) {
+                    const float x = (float)vr[lane + 64 * c];
+                    o[0][c] += sp[wave][0][t] * x;
+                    o[1][c] += sp[wave][1][t] * x;
+                }
             }
         }
+        const float lam = wave_lambda(a, h, lane);
+        const float r0 = l[0] > 0.0f ? 1.0f / l[0] : 0.0f, r1 = l[1] > 0.0f ? lam / l[1] : 0.0f;
+        float ss = 0.0f, y[NV];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float mn = fmaxf(m[j], wave_max(s[j]));
-            const float al = exp2f(m[j] - mn), p = lane < n ? exp2f(s[j] - mn) : 0.0f;
-            m[j] = mn;
-            l[j] = l[j] * al + wave_sum(p);
-            for (int c = 0; c < NV; ++c) o[j][c] *= al;
-            sp[wave][j][lane] = p;
+        for (int c = 0; c < NV; ++c) {
+            y[c] = o[0][c] * r0 - o[1][c] * r1;
+            ss += y[c] * y[c];
         }
-        for (int t = 0; t < n; ++t) {
-            const T *vr = v + (long long)(k0 + t) * a.ldv;
+        const float f = a.norm_w ? (1.0f - a.lambda_init) / sqrtf(wave_sum(ss) / (float)(2 * HD) + a.eps) : 1.0f;
+        T *out = (T *)a.out + (long long)b * a.bso + (long long)r * a.ldo + (long long)h * 2 * HD;
 #pragma unroll
-            for (int c = 0; c < NV; ++c) {
-                const float x = (float)vr[lane + 64 * c];
-                o[0][c] += sp[wave][0][t] * x;
-                o[1][c] += sp[wave][1][t] * x;
-            }
+        for (int c = 0; c < NV; ++c) {
+            const int i = lane + 64 * c;
+            out[i] = (T)(a.norm_w ? y[c] * f * a.norm_w[i] : y[c]);
         }
-    }
-    const float lam = wave_lambda(a, h, lane);
-    const float r0 = l[0] > 0.0f ? 1.0f / l[0] : 0.0f, r1 = l[1] > 0.0f ? lam / l[1] : 0.0f;
-    float ss = 0.0f, y[NV];
-#pragma unroll
-    for (int c = 0; c < NV; ++c) {
-        y[c] = o[0][c] * r0 - o[1][c] * r1;
-        ss += y[c] * y[c];
-    }
-    const float f = a.norm_w ? (1.0f - a.lambda_init) / sqrtf(wave_sum(ss) / (float)(2 * HD) + a.eps) : 1.0f;
-    T *out = (T *)a.out + (long long)b * a.bso + (long long)r * a.ldo + (long long)h * 2 * HD;
-#pragma unroll
-    for (int c = 0; c < NV; ++c) {
-        const int i = lane + 64 * c;
-        out[i] = (T)(a.norm_w ? y[c] * f * a.norm_w[i] : y[c]);
     }
 }
 
@@ -1005,7 +1007,7 @@ int launch_plan(const DiffAttnArgs &a, const DiffPlan &pl, hipStream_t st) {
 template <typename T, int HD>
 int launch_any(const DiffAttnArgs &a, hipStream_t st) {
     const unsigned long long n = (unsigned long long)a.B * a.Sq * a.nh;
-    TSN_LAUNCH((diff_attn_any_kernel<T, HD>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, a);
+    TSN_LAUNCH((diff_attn_any_kernel<T, HD>), dim3((unsigned)std::min<unsigned long long>((n + 3) / 4, 1 << 20)), dim3(256), 0, st, a);
     TSN_HIP_CHECK(hipGetLastError());
     return TSN_OK;
 }
@@ -1093,8 +1095,9 @@ int diff_attention_check(DiffAttnArgs &a) {
     TSN_REQUIRE(isfinite(a.scale) && a.scale >= 0.0f, "diff_attention: scale must be finite and not negative");
     TSN_REQUIRE(a.lambda_init >= 0.0f && a.lambda_init < 1.0f, "diff_attention: lambda_init must be in [0, 1)");
     TSN_REQUIRE(!a.norm_w || (isfinite(a.eps) && a.eps >= 0.0f), "diff_attention: eps must be finite and not negative");
-    TSN_REQUIRE(a.nh <= (1u << 12) && a.Sq < (1u << 30) && a.Sk < (1u << 30) &&
-                    (unsigned long long)a.B * a.Sq * a.nh < (1ULL << 31),
+    // the few-row kernel's tiles, 256 threads each, are less than 2^32 threads
+    TSN_REQUIRE(a.nh <= (1u << 12) && a.Sq < (1u << 30) && a.Sk < (1u << 30) && a.B < (1u << 24) &&
+                    ((unsigned long long)a.Sq * (a.nh / a.nkv) + 15) / 16 * a.nkv * a.B < (1ULL << 24),
                 "diff_attention: sizes beyond the launch grid");
     const uint32_t wq = 2 * a.nh * a.hd, wk = 2 * a.nkv * a.hd;
     if (!a.ldq) a.ldq = wq;
