@@ -1074,15 +1074,15 @@ def _need(what, arr, numel, itemsize=4, optional=False):
 def _hold(what, spec, arrays):
     """_need of a block operator's arrays, in the order of the spec's sizes(); the spec keeps them until a field changes"""
     key = bytes(spec)
-    kept = getattr(spec, "_kept", None)
+    kept = spec.__dict__.get("_kept")
     if kept is None or kept[0] != key:
         kept = spec._kept = key, spec.sizes()
-    for arr, (name, nbytes, optional) in zip(arrays, kept[1]):
+    for arr, size in zip(arrays, kept[1]):
         if arr is None:
-            if not optional:
-                raise ValueError("%s: %s: a device array is required" % (what, name))
-        elif type(arr) is not DeviceArray and not hasattr(arr, "p") or arr.nbytes < nbytes:
-            _need("%s: %s" % (what, name), arr, nbytes, 1)
+            if not size[2]:
+                raise ValueError("%s: %s: a device array is required" % (what, size[0]))
+        elif arr.__class__ is not DeviceArray and not hasattr(arr, "p") or arr.nbytes < size[1]:
+            _need("%s: %s" % (what, size[0]), arr, size[1], 1)
 
 
 def _p(arr):

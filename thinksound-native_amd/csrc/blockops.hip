@@ -24,7 +24,9 @@ inline bool passes_caches(size_t bytes) { return bytes >= ((size_t)192 << 20); }
 
 // What the kernels read of a call. freq: turns of a pair per position, in 64 bits: a position of 10^6 times a
 // frequency of one radian is off by a tenth of a radian in 32 bits. Pairs behind the last axis have frequency 0.
+// NP: pairs that fit (heads of up to 64 send a quarter of the frequencies, and half a microsecond less a launch).
 constexpr int MAX_PAIRS = 128;
+template <int NP>
 struct RopeKernelArgs {
     const void *x;
     const int32_t *pos;
@@ -34,11 +36,12 @@ struct RopeKernelArgs {
     unsigned start[4], dim[4];   // each axis' elements of a head
     unsigned total;              // elements of all axes
     int half_split;
-    double freq[MAX_PAIRS];
+    double freq[NP];
 };
 
 // pair p of a head: its axis and the positions of its two elements
-__device__ __forceinline__ void pair_at(const RopeKernelArgs &a, unsigned p, unsigned &axis, unsigned &e0, unsigned &e1) {
+template <int NP>
+__device__ __forceinline__ void pair_at(const RopeKernelArgs<NP> &a, unsigned p, unsigned &axis, unsigned &e0, unsigned &e1) {
     axis = 0;
     e0 = 2 * p;
     e1 = 2 * p + 1;
@@ -59,7 +62,7 @@ __device__ __forceinline__ void turn(double freq, int pos, float &cs, float &sn)
 
 // Any width, stride and alignment: a thread turns pair p of one row in every head, so its sine and cosine
 // are taken once.
-__global__ __launch_bounds__(256) void rope_axes_any_kernel(const RopeKernelArgs a) {
+__global__ __launch_bounds__(256) void rope_axes_any_kernel(const RopeKernelArgs<MAX_PAIRS> a) {
     const unsigned np = a.hd / 2;
     const long long n = (long long)a.rows * np;
     for (long long id = (long long)blockIdx.x * 256 + threadIdx.x; id < n; id += (long long)gridDim.x * 256) {
@@ -85,8 +88,8 @@ __global__ __launch_bounds__(256) void rope_axes_any_kernel(const RopeKernelArgs
 struct RopeChunks {
     unsigned rb, per_head, per_row, head_magic, row_magic;
 };
-template <typename T, bool HALF, bool ONCE>
-__global__ __launch_bounds__(256) void rope_axes_kernel(const RopeKernelArgs a, const RopeChunks c) {
+template <typename T, bool HALF, bool ONCE, int NP>
+__global__ __launch_bounds__(256) void rope_axes_kernel(const RopeKernelArgs<NP> a, const RopeChunks c) {
     constexpr int VE = 16 / sizeof(T), UN = 4;   // elements of a chunk; items in flight a thread
     typedef T vec __attribute__((ext_vector_type(VE)));
     extern __shared__ float2 table[];   // [row of the workgroup][pair]
@@ -440,59 +443,78 @@ int rope_axes_check(RopeAxesArgs &a) {
     return TSN_OK;
 }
 
-int launch_rope_axes(const RopeAxesArgs &c, hipStream_t st) {
-    RopeKernelArgs a{};
+namespace {
+
+// what the kernels read, but for the frequencies of pairs that NP does not hold
+template <int NP>
+RopeKernelArgs<NP> rope_kernel_args(const RopeAxesArgs &c) {
+    RopeKernelArgs<NP> a{};
     a.x = c.x; a.pos = c.pos; a.y = c.y; a.dt = c.dt;
     a.rows = c.rows; a.nh = c.nh; a.hd = c.hd; a.ldx = c.ldx; a.ldy = c.ldy; a.pos_rows = c.pos_rows; a.n_axes = c.n_axes;
     a.half_split = c.half_split;
     for (unsigned i = 0; i < c.n_axes; ++i) {
         a.start[i] = a.total;
         a.dim[i] = c.dim[i];
-        for (unsigned p = 0; p < c.dim[i] / 2; ++p) {
-            const double f = (double)c.fscale[i] * pow((double)c.base[i], -2.0 * p / c.dim[i]) / (2.0 * M_PI);
-            a.freq[a.total / 2 + p] = c.inverse ? -f : f;
-        }
+        // pair by pair times base^(-2/dim), in 64 bits of mantissa: 128 roundings are 2^-57, a pow a pair 1 us a call more
+        const long double ratio = c.dim[i] ? powl((long double)c.base[i], -2.0L / c.dim[i]) : 1.0L;
+        long double f = (c.inverse ? -1.0L : 1.0L) * c.fscale[i] / (2.0L * 3.14159265358979323846264338327950288L);
+        for (unsigned p = 0; p < c.dim[i] / 2; ++p, f *= ratio) a.freq[a.total / 2 + p] = (double)f;
         a.total += c.dim[i];
     }
+    return a;
+}
+
+template <typename T, int NP>
+int launch_rope_chunks(const RopeAxesArgs &c, const RopeChunks &k, hipStream_t st) {
+    const RopeKernelArgs<NP> a = rope_kernel_args<NP>(c);
+    const dim3 grid((c.rows + k.rb - 1) / k.rb);
+    const size_t lds = (size_t)k.rb * (c.hd / 2) * sizeof(float2);
+    const bool once = passes_caches((size_t)2 * c.rows * c.nh * c.hd * sizeof(T));
+    if (c.half_split) {
+        if (once) TSN_LAUNCH((rope_axes_kernel<T, true, true, NP>), grid, dim3(256), lds, st, a, k);
+        else TSN_LAUNCH((rope_axes_kernel<T, true, false, NP>), grid, dim3(256), lds, st, a, k);
+    } else {
+        if (once) TSN_LAUNCH((rope_axes_kernel<T, false, true, NP>), grid, dim3(256), lds, st, a, k);
+        else TSN_LAUNCH((rope_axes_kernel<T, false, false, NP>), grid, dim3(256), lds, st, a, k);
+    }
+    TSN_HIP_CHECK(hipGetLastError());
+    return TSN_OK;
+}
+template <typename T>
+int launch_rope_typed(const RopeAxesArgs &c, const RopeChunks &k, hipStream_t st) {
+    return c.hd <= 64 ? launch_rope_chunks<T, 32>(c, k, st) : launch_rope_chunks<T, MAX_PAIRS>(c, k, st);
+}
+
+} // namespace
+
+int launch_rope_axes(const RopeAxesArgs &c, hipStream_t st) {
     // whole chunks: aligned rows and heads, and for halves whole chunks of each half
     const unsigned ve = c.dt == DT_F32 ? 4 : 8;
+    unsigned total = 0;
     bool whole = (((uintptr_t)c.x | (uintptr_t)c.y) & 15) == 0 && c.ldx % ve == 0 && c.ldy % ve == 0 && c.hd % ve == 0;
-    if (c.half_split)
-        for (unsigned i = 0; i < c.n_axes; ++i) whole = whole && c.dim[i] % (2 * ve) == 0;
+    for (unsigned i = 0; i < c.n_axes; ++i) {
+        whole = whole && (!c.half_split || c.dim[i] % (2 * ve) == 0);
+        total += c.dim[i];
+    }
     if (whole) {
         RopeChunks k{};
-        k.per_head = c.half_split ? (a.total / 2 + (c.hd - a.total)) / ve : c.hd / ve;
+        k.per_head = c.half_split ? (total / 2 + (c.hd - total)) / ve : c.hd / ve;
         k.per_row = c.nh * k.per_head;
-        const unsigned un = 4;
-        // rows that give a workgroup's threads `un` items each, but no more than leave every CU eight workgroups
+        // rows that give a workgroup's threads four items each, but no more than leave every CU eight workgroups
         const unsigned long long fill = c.rows / 2048 + 1;
-        k.rb = (unsigned)std::max<unsigned long long>(1, std::min<unsigned long long>({256 * un / k.per_row, fill, 16384 / c.hd}));
+        k.rb = (unsigned)std::max<unsigned long long>(1, std::min<unsigned long long>({1024 / k.per_row, fill, 16384 / c.hd}));
         k.rb = std::max(k.rb, c.rows >> 23);   // a launch has less than 2^32 threads
         // i / d = umulhi(i, magic) while i * d < 2^32
         auto magic = [](unsigned d) { return d == 1 ? 0u : (unsigned)((0x100000000ULL + d - 1) / d); };
         k.head_magic = magic(k.per_head);
         k.row_magic = magic(k.per_row);
         const unsigned long long most = (unsigned long long)k.rb * k.per_row;
-        whole = k.per_head > 1 && most * k.per_row < (1ULL << 32) && k.rb <= 16384 / c.hd;
-        if (whole) {
-            const dim3 grid((c.rows + k.rb - 1) / k.rb);
-            const size_t lds = (size_t)k.rb * (c.hd / 2) * sizeof(float2);
-            const bool once = passes_caches((size_t)2 * c.rows * c.nh * c.hd * elem_bytes(c.dt));
-#define ROPE_AS(T, HALF)                                                                                \
-    if (once) TSN_LAUNCH((rope_axes_kernel<T, HALF, true>), grid, dim3(256), lds, st, a, k);            \
-    else TSN_LAUNCH((rope_axes_kernel<T, HALF, false>), grid, dim3(256), lds, st, a, k)
-#define ROPE(T)                                   \
-    if (c.half_split) { ROPE_AS(T, true); }       \
-    else { ROPE_AS(T, false); }
-            if (c.dt == DT_F32) { ROPE(float); }
-            else if (c.dt == DT_F16) { ROPE(half_t); }
-            else { ROPE(bf16_t); }
-#undef ROPE
-#undef ROPE_AS
-            TSN_HIP_CHECK(hipGetLastError());
-            return TSN_OK;
+        if (k.per_head > 1 && most * k.per_row < (1ULL << 32) && k.rb <= 16384 / c.hd) {
+            if (c.dt == DT_F32) return launch_rope_typed<float>(c, k, st);
+            return c.dt == DT_F16 ? launch_rope_typed<half_t>(c, k, st) : launch_rope_typed<bf16_t>(c, k, st);
         }
     }
+    const RopeKernelArgs<MAX_PAIRS> a = rope_kernel_args<MAX_PAIRS>(c);
     const unsigned long long n = (unsigned long long)c.rows * (c.hd / 2);
     TSN_LAUNCH(rope_axes_any_kernel, dim3((unsigned)std::min<unsigned long long>((n + 255) / 256, 1 << 20)), dim3(256), 0, st, a);
     TSN_HIP_CHECK(hipGetLastError());
