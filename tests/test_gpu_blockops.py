@@ -532,6 +532,28 @@ def test_diff_attention_lambda(tsn, rt, lambda_init):
     attn_case(tsn, rt, F16, 2, 40, 300, 4, 4, 64, lam_heads=4, lambda_init=lambda_init)
 
 
+@pytest.mark.parametrize("hd", [64, 32])
+@pytest.mark.parametrize("B,Sq,Sk,nkv,pad", [(2, 5, 300, 2, 0), (2, 5, 300, 2, 1), (2, 3, 9000, 1, 0), (8, 1300, 700, 16, 0), (2, 900, 3000, 2, 0)])
+def test_diff_attention_no_keys_no_eps(tsn, rt, hd, B, Sq, Sk, nkv, pad):
+    """rows that see no key are zeros with an eps of 0 too: a sample without keys, and causal rows before the first"""
+    w = 2 * nkv * hd
+    r = rng(Sk + hd)
+    q = rt.array(enc(r.standard_normal((B * Sq, w + pad)), F16))
+    k = rt.array(enc(r.standard_normal((B * Sk, w)), F16))
+    lam, nw = rt.array(np.zeros((1, 4, hd), np.float32)), rt.array(np.ones(2 * hd, np.float32))
+    kl = [0] + [Sk] * (B - 2) + [Sq - 2]
+    klb, o = rt.array(np.asarray(kl, np.int32)), rt.array(np.full((B * Sq, w), np.nan, np.float16))
+    rt.diff_attention(tsn.diff_attn_spec(F16, B, Sq, Sk, nkv, nkv, hd, causal=True, eps=0.0, ldq=w + pad), q, k, k, lam, nw, None, klb, o)
+    rt.sync()
+    got = o.numpy().reshape(B, Sq, w)
+    for b in range(B):
+        empty = max(0, Sq - min(kl[b], Sk))   # lengths past Sk are Sk
+        assert (got[b, :empty] == 0).all()
+        assert np.isfinite(got[b, empty:]).all() and (got[b, empty + 1:] != 0).any(-1).all()
+    for t in (q, k, lam, nw, klb, o):
+        t.free()
+
+
 def test_diff_attention_far_offsets(tsn, rt):
     """samples and rows of a cache that lie more than 2^32 bytes from its start"""
     dt, hd, Sk, nh = F16, 64, 130, 2

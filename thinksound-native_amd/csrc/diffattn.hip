@@ -35,6 +35,12 @@ __device__ __forceinline__ float wave_lambda(const DiffAttnArgs &a, int h, int l
     return expf(d1) - expf(d2) + a.lambda_init;
 }
 
+// what the RMS norm multiplies a row of these squares with; a row without keys stays zero also where eps is
+template <int HD>
+__device__ __forceinline__ float rms_factor(const DiffAttnArgs &a, float squares) {
+    return squares == 0.0f ? 0.0f : (1.0f - a.lambda_init) / sqrtf(squares / (float)(2 * HD) + a.eps);
+}
+
 // Any stride and alignment: one wave a row and head. A block of 64 keys at a time, lane j takes the scores of key j;
 // the probabilities go through LDS, then the lanes take the columns of V.
 template <typename T, int HD>
@@ -99,7 +105,7 @@ __global__ __launch_bounds__(256) void diff_attn_any_kernel(const DiffAttnArgs a
             y[c] = o[0][c] * r0 - o[1][c] * r1;
             ss += y[c] * y[c];
         }
-        const float f = a.norm_w ? (1.0f - a.lambda_init) / sqrtf(wave_sum(ss) / (float)(2 * HD) + a.eps) : 1.0f;
+        const float f = a.norm_w ? rms_factor<HD>(a, wave_sum(ss)) : 1.0f;
         T *out = (T *)a.out + (long long)b * a.bso + (long long)r * a.ldo + (long long)h * 2 * HD;
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
@@ -572,7 +578,7 @@ struct Wide {
         ss = pair_sum(ss);
         if (ro.qi >= nq) return;
         if (a.norm_w) {
-            const float f = (1.0f - a.lambda_init) / sqrtf(ss / (float)(2 * HD) + a.eps);
+            const float f = rms_factor<HD>(a, ss);
             const float *nw = a.norm_w + col0;
 #pragma unroll
             for (int d = 0; d < L::DT; ++d)
@@ -845,7 +851,7 @@ struct Few {
             red[kw * 64] = quad_sum(ss);
             block_barrier();
             ss = ((red[0] + red[64]) + red[128]) + red[192];
-            const float fn = (1.0f - a.lambda_init) / sqrtf(ss / (float)(2 * HD) + a.eps);
+            const float fn = rms_factor<HD>(a, ss);
 #pragma unroll
             for (int i = 0; i < NQ; ++i) y[0][i] = y[0][i] * fn * nw[i];
         }
@@ -990,7 +996,7 @@ __global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs 
     const float ss = row_sum((y[0] * y[0] + y[1] * y[1]) + (y[2] * y[2] + y[3] * y[3]));
     if (!in) return;
     if (a.norm_w) {
-        const float f = (1.0f - a.lambda_init) / sqrtf(ss / (float)(2 * HD) + a.eps);
+        const float f = rms_factor<HD>(a, ss);
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = y[e] * f * a.norm_w[4 * lane + e];
     }
