@@ -37,6 +37,7 @@ def rope(tsn, x=BASE, pos=BASE + (1 << 36), y=BASE + (1 << 35), **kw):
     (dict(rows=0), "empty"), (dict(nh=0), "empty"), (dict(hd=0), "empty"),
     (dict(hd=63), "even"), (dict(hd=258), "256"),
     (dict(n_axes=0), "axes"), (dict(n_axes=5), "axes"),
+    (dict(rows=1 << 31), "rows"), (dict(rows=(1 << 31) - 1, dtype=0, ldx=(1 << 31) + 8, x=1 << 20, y=BASE), "overlap"),
     (dict(dim=(1, 23)), "even"), (dict(dim=(1, 26)), "more than hd"), (dict(dim=(0, 0xFFFFFFFE)), "more than hd"),
     (dict(base=(0, 0.0)), "base"), (dict(base=(2, -1.0)), "base"), (dict(base=(1, float("nan"))), "base"),
     (dict(fscale=(0, float("inf"))), "finite"),
@@ -76,6 +77,7 @@ def attn(tsn, q=BASE, k=BASE + (1 << 36), v=BASE + (2 << 36), lam=BASE + (3 << 3
     (dict(ldq=1023), "row stride", 1), (dict(ldk=511), "row stride", 1), (dict(ldv=500), "row stride", 1), (dict(ldo=1000), "row stride", 1),
     (dict(ldk=(1 << 22) + 8), "row stride", 1), (dict(bsk=1 << 40), "sample stride", 1),
     (dict(bso=39 * 1024), "samples of out", 1), (dict(bso=1024, ldo=2048), NULL_RT, 1),
+    (dict(B=1 << 23, Sq=1, nh=1, nkv=1, bsq=(1 << 40) - 8, bsk=1 << 8), "overlaps an input", 1),
     (dict(q=BASE + 1), "aligned", 1), (dict(lam=BASE + (3 << 36) + 2), "aligned", 1),
     (dict(out=BASE), "overlaps an input", 1), (dict(out=BASE + (1 << 36) + 1024), "overlaps an input", 1),
     (dict(out=BASE + (2 << 36) - 2048), "overlaps an input", 1),
@@ -102,6 +104,7 @@ def norm(tsn, x=BASE, f=BASE + (1 << 36), mod=BASE + (2 << 36), pw=None, pb=None
     (dict(post=3), "norm kind", 1), (dict(pre=-1), "norm kind", 1),
     (dict(rows=0), "empty", 1), (dict(H=0), "empty", 1), (dict(H=16385), "16384", 3),
     (dict(x_scale=float("nan")), "scales", 1), (dict(f_scale=float("inf")), "scales", 1),
+    (dict(rows=1 << 31), "rows", 1), (dict(rows=(1 << 31) - 1, ldf=(1 << 31) + 8, f=1 << 20, xo=BASE, y=None, mod=None, gate=-1, shift=-1, scale=-1), "x_out overlaps f", 1),
     (dict(post_eps=-1.0), "eps", 1), (dict(pre_eps=float("nan")), "eps", 1),
     (dict(gate=3), "chunk", 1), (dict(shift=-2), "chunk", 1), (dict(scale=7), "chunk", 1), (dict(mod=None), "chunk", 1),
     (dict(ldx=99), "stride", 1), (dict(ldf=1), "stride", 1), (dict(ldo=99), "stride", 1), (dict(ldy=50), "stride", 1),

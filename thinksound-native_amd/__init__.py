@@ -408,7 +408,7 @@ def rope_axes_spec(dtype, rows, nh, hd, dims, bases, fscales=None, ldx=0, ldy=0,
         raise ValueError("rope_axes: one to four axes, a base (and scale) for each")
     a4 = lambda t, v: (t * 4)(*v, *([0] * (4 - n)))  # noqa: E731
     return RopeAxesSpec(dtype, rows, nh, hd, ldx, ldy, pos_rows, n, a4(ctypes.c_uint32, dims), a4(ctypes.c_float, bases),
-                        a4(ctypes.c_float, fscales or [1.0] * n), int(half_split), int(inverse))
+                        a4(ctypes.c_float, [1.0] * n if fscales is None else fscales), int(half_split), int(inverse))
 
 
 def diff_attn_spec(dtype, B, Sq, Sk, nh, nkv, hd, causal=False, scale=None, lambda_init=0.8, eps=1e-5, lam_heads=1,

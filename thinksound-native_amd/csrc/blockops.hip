@@ -419,6 +419,7 @@ int rope_axes_check(RopeAxesArgs &a) {
     TSN_REQUIRE(a.x && a.pos && a.y, "rope_axes: null tensor");
     TSN_REQUIRE(is_elem(a.dt), "rope_axes: dtype f32, f16 or bf16");
     TSN_REQUIRE(a.rows > 0 && a.nh > 0 && a.hd > 0, "rope_axes: empty shape");
+    TSN_REQUIRE(a.rows < (1u << 31), "rope_axes: 2^31 rows or more");
     TSN_REQUIRE(a.hd % 2 == 0 && a.hd <= 2 * MAX_PAIRS, "rope_axes: hd must be even and at most 256");
     TSN_REQUIRE(a.n_axes >= 1 && a.n_axes <= 4, "rope_axes: one to four axes");
     unsigned long long total = 0;
@@ -526,6 +527,7 @@ int gate_add_norm_check(GateNormArgs &a) {
     TSN_REQUIRE(is_elem(a.xdt) && is_elem(a.fdt) && is_elem(a.ydt), "gate_add_norm: dtypes f32, f16 or bf16");
     TSN_REQUIRE(a.post >= NORM_NONE && a.post <= NORM_LN && a.pre >= NORM_NONE && a.pre <= NORM_LN, "gate_add_norm: norm kind");
     TSN_REQUIRE(a.rows > 0 && a.H > 0, "gate_add_norm: empty shape");
+    TSN_REQUIRE(a.rows < (1u << 31), "gate_add_norm: 2^31 rows or more");
     if (a.H > 16384) {
         set_error("gate_add_norm: H above 16384");
         return TSN_ERR_UNSUPPORTED;

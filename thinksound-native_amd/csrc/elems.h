@@ -40,7 +40,9 @@ __device__ __forceinline__ void store8(T *p, const floatx8 &v, ONCE) {   // true
 struct Window {
     const void *p;
     unsigned long long width, ld, rows, bs, samples;
-    unsigned long long end() const { return (unsigned long long)p + (samples - 1) * bs + (rows - 1) * ld + width; }
+    unsigned __int128 end() const {   // strides and counts of any size: more than 64 bits
+        return (unsigned __int128)(unsigned long long)p + (unsigned __int128)(samples - 1) * bs + (unsigned __int128)(rows - 1) * ld + width;
+    }
 };
 inline Window window(const void *p, size_t elem, unsigned long long width, unsigned long long ld,
                      unsigned long long rows, unsigned long long bs = 0, unsigned long long samples = 1) {
