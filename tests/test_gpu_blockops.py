@@ -464,6 +464,9 @@ CUTS = [
     (3, 1000, 2500, 24, 24, False, "ragged", (0, 11, 23)),
     (1, 2500, 2500, 8, 8, True, None, (2, 7)),         # causal tiles, heads round the XCDs
     (4, 500, 500, 6, 2, True, "ragged", (0, 5)),
+    (5, 1300, 1500, 40, 10, True, "ragged", (0, 23, 39)),      # causal tiles by length: all resident at once
+    (33, 700, 700, 16, 8, True, "some empty", (0, 9, 15)),     # more of them, samples without rows and without keys
+    (3, 1500, 400, 48, 48, True, "ragged", (0, 47)),           # more rows than keys: tiles without keys
 ]
 
 
@@ -474,7 +477,7 @@ def test_diff_attention_cuts(tsn, rt, dt, hd, B, Sq, Sk, nh, nkv, causal, kl, he
     lens = None if kl is None else [int(t) for t in r.integers(Sk // 4, Sk + 1, B)]
     ql = None
     if kl == "some empty":
-        lens[3], lens[65], lens[69] = 0, 1, 0
+        lens[3], lens[B - 5], lens[B - 1] = 0, 1, 0
         ql = [int(t) for t in r.integers(0, Sq + 1, B)]
     attn_case(tsn, rt, dt, B, Sq, Sk, nh, nkv, hd, causal, ql, lens, junk=None if kl is None else np.nan, heads=heads)
 

@@ -403,6 +403,7 @@ struct DiffPlan {
     int tiles, units;   // of all heads and samples; of a tile (by Sk)
     int full, shared;
     int by_len;         // full = 0 and lengths are given: the units are counted by them
+    int ranked;         // causal, full = tiles and lengths are given: the tiles are ordered by them
     float *o;           // [piece][row of the tile][map][2 HD]: products with V, not divided
     float4 *st;         // [piece][row of the tile]: reference and sum of each map
 };
@@ -411,6 +412,16 @@ struct Share {   // shared workgroup p's units begin at p*q + min(p, r)
     __device__ __forceinline__ unsigned begin(unsigned p) const { return p * q + min(p, r); }
     __device__ __forceinline__ unsigned holder(unsigned u) const { return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q; }
 };
+// sum over the lanes up to this one: within rows of 16, then from row to row
+__device__ __forceinline__ unsigned lane_prefix(unsigned v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
 // The samples' units by their lengths, 64 samples at a time: lane i looks at sample b0 + i, which has nkv * tiles * n
 // units (tiles of a head, units of a tile)
 template <int TR, int KB>
@@ -425,14 +436,7 @@ struct ByLen {
         tiles = (int)(((unsigned)nq * (a.nh / a.nkv) + TR - 1) / TR);
         n = (unsigned)max(1, (nk + KB - 1) / KB);
         own = from + lane < (int)a.B ? a.nkv * tiles * n : 0;
-        unsigned v = own;   // sum over the lanes up to this one: within rows of 16, then from row to row
-        v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
-        v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-        v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-        v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-        v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
-        v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-        upto = v;
+        upto = lane_prefix(own);
     }
     __device__ __forceinline__ unsigned all() const { return __builtin_amdgcn_readlane(upto, 63); }
     // of all samples; the first 64 are being looked at before and after
@@ -488,6 +492,42 @@ __device__ __forceinline__ Part part_at(const DiffAttnArgs &a, const DiffPlan &p
     p.u1 = (int)min((unsigned)p.n, p.u0 + (end - u));
     p.place = (p.b * (int)a.nkv + p.g) * pl.ntile + tile_order(a, pl.ntile, p.tile) - pl.full;
     return p;
+}
+
+// Every other block of n workgroups of `all` turned round: n CUs get one of each block, the one with the longest tile of a
+// block the shortest of the next
+__device__ __forceinline__ int mirrored(int i, int n, int all) {
+    const int block = i / n, first = block * n;
+    return block & 1 ? first + min(n, all - first) - 1 - (i - first) : i;
+}
+// Causal tiles of up to 64 samples of unequal length, longest first over all: a sample's tiles end at level
+// nk*G/TR, one level apart. Sets b, nq, nk, g, tile and returns whether there is a tile of rank i.
+template <int TR, int WAVES>
+__device__ __forceinline__ bool ranked_part(const DiffAttnArgs &a, const DiffPlan &pl, Part &p, int i, int lane) {
+    const int b = min(lane, (int)a.B - 1), G = (int)(a.nh / a.nkv);
+    const int nq = q_rows(a, b), nk = kv_rows(a, b);
+    const int tiles = lane < (int)a.B ? (int)(((unsigned)nq * G + TR - 1) / TR) : 0, top = (int)((unsigned)nk * G / TR);
+    auto from = [&](int level) {   // tiles of the level and above, up to and with the lane's sample
+        return lane_prefix(a.nkv * (unsigned)min(max(top - level + 1, 0), tiles));
+    };
+    int lo = -(int)pl.ntile, hi = (int)(a.Sk * G / TR);   // every tile is at lo or above, none above hi
+    const int n = (int)__builtin_amdgcn_readlane(from(lo), 63);
+    if (n <= WAVES * 256) i = mirrored(i, 256, pl.full);
+    if (i >= n) return false;
+    while (lo < hi) {   // the highest level with more than i tiles from it on
+        const int mid = lo + (hi - lo + 1) / 2;
+        if ((int)__builtin_amdgcn_readlane(from(mid), 63) > i) lo = mid;
+        else hi = mid - 1;
+    }
+    const unsigned above = __builtin_amdgcn_readlane(from(lo + 1), 63), rest = (unsigned)i - above;
+    const unsigned own = top - lo >= 0 && top - lo < tiles ? a.nkv : 0, upto = lane_prefix(own);
+    const int at = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(upto > rest)) - 1;
+    p.b = at;
+    p.nq = __builtin_amdgcn_readlane(nq, at);
+    p.nk = __builtin_amdgcn_readlane(nk, at);
+    p.g = (int)(rest - __builtin_amdgcn_readlane(upto - own, at));
+    p.tile = __builtin_amdgcn_readlane(tiles - 1 - (top - lo), at);
+    return true;
 }
 
 // A workgroup's worker: 128 rows, 32 a wave. The four waves share K and V tiles of 64 keys, two stages in LDS: the next is
@@ -879,25 +919,31 @@ __global__ __launch_bounds__(256, A::WAVES) void diff_attn_kernel(const DiffAttn
     __shared__ __attribute__((aligned(1024))) char smem[A::LDS];
     const int lane = threadIdx.x & 63, nkv = (int)a.nkv;
     if ((int)blockIdx.x < pl.full) {
-        // workgroups go round the 8 XCDs in turn. A head's tiles stay on one, for its L2; heads go round too, so that a
-        // short sample's are not all on one; causal tiles the longest first, over all the XCD's heads
-        const int heads = nkv * (int)a.B;
-        int bg, i;
-        if (heads % 8 == 0 && pl.full == pl.tiles) {
-            const int per = heads / 8, idx = (int)blockIdx.x >> 3;
-            i = a.causal ? idx / per : idx % pl.ntile;
-            bg = (a.causal ? idx - i * per : idx / pl.ntile) * 8 + ((int)blockIdx.x & 7);
-        } else {
-            const int t = (int)xcd_remap(blockIdx.x, pl.full);
-            bg = t / pl.ntile;
-            i = t - bg * pl.ntile;
-        }
         Part p;
-        p.b = bg / nkv;
-        p.g = bg - p.b * nkv;
-        p.tile = tile_order(a, pl.ntile, i);
-        p.nq = q_rows(a, p.b);
-        p.nk = kv_rows(a, p.b);
+        if (pl.ranked) {
+            if (!ranked_part<A::TR, A::WAVES>(a, pl, p, (int)blockIdx.x, lane)) return;
+        } else {
+            // workgroups go round the 8 XCDs in turn. A head's tiles stay on one, for its L2; heads go round too, so that a
+            // short sample's are not all on one; causal tiles the longest first, over all the XCD's heads
+            const int heads = nkv * (int)a.B;
+            int bg, i;
+            if (heads % 8 == 0 && pl.full == pl.tiles) {
+                const int per = heads / 8, n = pl.full / 8;
+                int idx = (int)blockIdx.x >> 3;
+                if (a.causal && n <= A::WAVES * 32) idx = mirrored(idx, 32, n);
+                i = a.causal ? idx / per : idx % pl.ntile;
+                bg = (a.causal ? idx - i * per : idx / pl.ntile) * 8 + ((int)blockIdx.x & 7);
+            } else {
+                const int t = (int)xcd_remap(blockIdx.x, pl.full);
+                bg = t / pl.ntile;
+                i = t - bg * pl.ntile;
+            }
+            p.b = bg / nkv;
+            p.g = bg - p.b * nkv;
+            p.tile = tile_order(a, pl.ntile, i);
+            p.nq = q_rows(a, p.b);
+            p.nk = kv_rows(a, p.b);
+        }
         p.u0 = 0;
         p.u1 = pl.units;
         A::run(a, pl, smem, p, -1);
@@ -1069,6 +1115,8 @@ DiffChoice choose(const DiffAttnArgs &a) {
             d.pl.full = full;
             d.pl.shared = shared;
             d.pl.by_len = full == 0 && (a.q_len || a.kv_len);
+            d.pl.ranked = tr == 128 && full == p.tiles && a.causal && (a.q_len || a.kv_len) && a.B <= 64 &&
+                          (unsigned long long)a.Sk * (a.nh / a.nkv) < (1ULL << 30);
             if (d.bytes() > ((size_t)256 << 20)) return;
             best = d;
             least = us;
