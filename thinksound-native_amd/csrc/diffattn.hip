@@ -403,7 +403,7 @@ struct DiffPlan {
     int tiles, units;   // of all heads and samples; of a tile (by Sk)
     int full, shared;
     int by_len;         // full = 0 and lengths are given: the units are counted by them
-    int ranked;         // causal, full = tiles and lengths are given: the tiles are ordered by them
+    int ranked;         // causal, full = tiles, lengths that differ or heads that do not go round the XCDs: see ranked_part
     float *o;           // [piece][row of the tile][map][2 HD]: products with V, not divided
     float4 *st;         // [piece][row of the tile]: reference and sum of each map
 };
@@ -501,18 +501,21 @@ __device__ __forceinline__ int mirrored(int i, int n, int all) {
     return block & 1 ? first + min(n, all - first) - 1 - (i - first) : i;
 }
 // Causal tiles of up to 64 samples of unequal length, longest first over all: a sample's tiles end at level
-// nk*G/TR, one level apart. Sets b, nq, nk, g, tile and returns whether there is a tile of rank i.
+// nk*G/TR, one level apart. Sets b, nq, nk, g, tile and returns whether there is a tile of the workgroup's rank. Samples
+// of a multiple of eight heads give each XCD an eighth of them, and it ranks its own.
 template <int TR, int WAVES>
-__device__ __forceinline__ bool ranked_part(const DiffAttnArgs &a, const DiffPlan &pl, Part &p, int i, int lane) {
+__device__ __forceinline__ bool ranked_part(const DiffAttnArgs &a, const DiffPlan &pl, Part &p, int lane) {
+    const int xcds = a.nkv % 8 == 0 ? 8 : 1, nkv = (int)a.nkv / xcds, cus = 256 / xcds, all = pl.full / xcds;
+    int i = (int)blockIdx.x / xcds;
     const int b = min(lane, (int)a.B - 1), G = (int)(a.nh / a.nkv);
     const int nq = q_rows(a, b), nk = kv_rows(a, b);
     const int tiles = lane < (int)a.B ? (int)(((unsigned)nq * G + TR - 1) / TR) : 0, top = (int)((unsigned)nk * G / TR);
     auto from = [&](int level) {   // tiles of the level and above, up to and with the lane's sample
-        return lane_prefix(a.nkv * (unsigned)min(max(top - level + 1, 0), tiles));
+        return lane_prefix((unsigned)(nkv * min(max(top - level + 1, 0), tiles)));
     };
     int lo = -(int)pl.ntile, hi = (int)(a.Sk * G / TR);   // every tile is at lo or above, none above hi
     const int n = (int)__builtin_amdgcn_readlane(from(lo), 63);
-    if (n <= WAVES * 256) i = mirrored(i, 256, pl.full);
+    if (n <= WAVES * cus) i = mirrored(i, cus, all);
     if (i >= n) return false;
     while (lo < hi) {   // the highest level with more than i tiles from it on
         const int mid = lo + (hi - lo + 1) / 2;
@@ -520,12 +523,12 @@ __device__ __forceinline__ bool ranked_part(const DiffAttnArgs &a, const DiffPla
         else hi = mid - 1;
     }
     const unsigned above = __builtin_amdgcn_readlane(from(lo + 1), 63), rest = (unsigned)i - above;
-    const unsigned own = top - lo >= 0 && top - lo < tiles ? a.nkv : 0, upto = lane_prefix(own);
+    const unsigned own = top - lo >= 0 && top - lo < tiles ? nkv : 0, upto = lane_prefix(own);
     const int at = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(upto > rest)) - 1;
     p.b = at;
     p.nq = __builtin_amdgcn_readlane(nq, at);
     p.nk = __builtin_amdgcn_readlane(nk, at);
-    p.g = (int)(rest - __builtin_amdgcn_readlane(upto - own, at));
+    p.g = (int)(rest - __builtin_amdgcn_readlane(upto - own, at)) * xcds + (int)blockIdx.x % xcds;
     p.tile = __builtin_amdgcn_readlane(tiles - 1 - (top - lo), at);
     return true;
 }
@@ -921,7 +924,7 @@ __global__ __launch_bounds__(256, A::WAVES) void diff_attn_kernel(const DiffAttn
     if ((int)blockIdx.x < pl.full) {
         Part p;
         if (pl.ranked) {
-            if (!ranked_part<A::TR, A::WAVES>(a, pl, p, (int)blockIdx.x, lane)) return;
+            if (!ranked_part<A::TR, A::WAVES>(a, pl, p, lane)) return;
         } else {
             // workgroups go round the 8 XCDs in turn. A head's tiles stay on one, for its L2; heads go round too, so that a
             // short sample's are not all on one; causal tiles the longest first, over all the XCD's heads
@@ -1115,7 +1118,7 @@ DiffChoice choose(const DiffAttnArgs &a) {
             d.pl.full = full;
             d.pl.shared = shared;
             d.pl.by_len = full == 0 && (a.q_len || a.kv_len);
-            d.pl.ranked = tr == 128 && full == p.tiles && a.causal && (a.q_len || a.kv_len) && a.B <= 64 &&
+            d.pl.ranked = tr == 128 && full == p.tiles && a.causal && (a.q_len || a.kv_len || heads % 8) && a.B <= 64 &&
                           (unsigned long long)a.Sk * (a.nh / a.nkv) < (1ULL << 30);
             if (d.bytes() > ((size_t)256 << 20)) return;
             best = d;
