@@ -404,6 +404,7 @@ struct DiffPlan {
     int full, shared;
     int by_len;         // full = 0 and lengths are given: the units are counted by them
     int ranked;         // causal, full = tiles, lengths that differ or heads that do not go round the XCDs: see ranked_part
+    int groups;         // workgroups of a tile that join its rows
     float *o;           // [piece][row of the tile][map][2 HD]: products with V, not divided
     float4 *st;         // [piece][row of the tile]: reference and sum of each map
 };
@@ -967,11 +968,11 @@ __global__ __launch_bounds__(256, A::WAVES) void diff_attn_kernel(const DiffAttn
 // PG groups of lanes take a row's pieces in turn (as many as a workgroup has beside few rows) and are merged in LDS.
 template <typename T, int HD, int TR, int KB, int PG>
 __global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs a, const DiffPlan pl) {
-    constexpr int LR = HD / 2, RPW = 256 / LR / PG, GROUPS = TR / RPW;   // rows of a workgroup; workgroups of a tile
+    constexpr int LR = HD / 2, RPW = 256 / LR / PG;   // rows of a workgroup
     __shared__ float4 part[PG > 1 ? 2 * 256 : 1];
     __shared__ float4 stat[PG > 1 ? 256 / LR : 1];
     const int lane = threadIdx.x & (LR - 1), team = (int)threadIdx.x / LR, rr = team % RPW, pg = team / RPW;
-    const int ts = (int)(blockIdx.x / GROUPS), r0 = (int)(blockIdx.x % GROUPS) * RPW, r = r0 + rr;
+    const int ts = (int)(blockIdx.x / (unsigned)pl.groups), r0 = (int)(blockIdx.x - (unsigned)ts * pl.groups) * RPW, r = r0 + rr;
     const int t = pl.full + ts, bg = t / pl.ntile, nkv = (int)a.nkv;
     const int b = bg / nkv, g = bg - b * nkv, G = (int)(a.nh / a.nkv);
     const int tile = tile_order(a, pl.ntile, t - bg * pl.ntile);
@@ -996,6 +997,13 @@ __global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs 
     const RowOf ro = row_of(tile * TR + r, G);
     const bool in = ro.qi < nq;
     const int h = g * G + (in ? ro.hg : 0);
+    // loaded beside the pieces
+    const float *lv = a.lam + (a.lam_heads > 1 ? (long long)h * 4 * HD : 0) + 2 * lane;
+    const float2 lq1 = make_float2(lv[0], lv[1]), lk1 = make_float2(lv[HD], lv[HD + 1]);
+    const float2 lq2 = make_float2(lv[2 * HD], lv[2 * HD + 1]), lk2 = make_float2(lv[3 * HD], lv[3 * HD + 1]);
+    float nw[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) nw[e] = a.norm_w ? a.norm_w[4 * lane + e] : 1.0f;
     float m[2] = {-1e30f, -1e30f}, l[2] = {0.0f, 0.0f};
     float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
     // one more part: the larger reference, what was before scaled to it
@@ -1037,8 +1045,7 @@ __global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs 
         }
         return v;
     };
-    const float *lv = a.lam + (a.lam_heads > 1 ? (long long)h * 4 * HD : 0) + 2 * lane;
-    const float d1 = row_sum(lv[0] * lv[HD] + lv[1] * lv[HD + 1]), d2 = row_sum(lv[2 * HD] * lv[3 * HD] + lv[2 * HD + 1] * lv[3 * HD + 1]);
+    const float d1 = row_sum(lq1.x * lk1.x + lq1.y * lk1.y), d2 = row_sum(lq2.x * lk2.x + lq2.y * lk2.y);
     const float lam = expf(d1) - expf(d2) + a.lambda_init;
     const float i0 = l[0] > 0.0f ? 1.0f / l[0] : 0.0f, i1 = l[1] > 0.0f ? lam / l[1] : 0.0f;
     float y[4] = {o[0].x * i0 - o[1].x * i1, o[0].y * i0 - o[1].y * i1, o[0].z * i0 - o[1].z * i1, o[0].w * i0 - o[1].w * i1};
@@ -1047,7 +1054,7 @@ __global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs 
     if (a.norm_w) {
         const float f = rms_factor<HD>(a, ss);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = y[e] * f * a.norm_w[4 * lane + e];
+        for (int e = 0; e < 4; ++e) y[e] = y[e] * f * nw[e];
     }
     T *out = (T *)a.out + (long long)b * a.bso + (long long)ro.qi * a.ldo + (long long)h * 2 * HD + 4 * lane;
     *(int2 *)out = make_int2(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]));
@@ -1060,12 +1067,14 @@ bool chunked(const DiffAttnArgs &a) {
 }
 
 template <typename T, int HD, typename A>
-int launch_plan(const DiffAttnArgs &a, const DiffPlan &pl, hipStream_t st) {
+int launch_plan(const DiffAttnArgs &a, DiffPlan &pl, hipStream_t st) {
     TSN_LAUNCH((diff_attn_kernel<T, HD, A>), dim3((unsigned)(pl.full + pl.shared)), dim3(256), 0, st, a, pl);
     TSN_HIP_CHECK(hipGetLastError());
     if (pl.shared > 0) {
-        constexpr int PG = A::TR == 16 ? 8 : 1, GROUPS = A::TR * PG * HD / 512;
-        TSN_LAUNCH((diff_attn_join_kernel<T, HD, A::TR, A::KB, PG>), dim3((unsigned)(pl.tiles - pl.full) * GROUPS), dim3(256), 0, st, a, pl);
+        constexpr int PG = A::TR == 16 ? 8 : 1, RPW = 512 / HD / PG;
+        const long long rows = std::min<long long>(A::TR, (long long)a.Sq * (a.nh / a.nkv));   // a tile has at most
+        pl.groups = (int)((rows + RPW - 1) / RPW);
+        TSN_LAUNCH((diff_attn_join_kernel<T, HD, A::TR, A::KB, PG>), dim3((unsigned)(pl.tiles - pl.full) * pl.groups), dim3(256), 0, st, a, pl);
         TSN_HIP_CHECK(hipGetLastError());
     }
     return TSN_OK;
