@@ -3,6 +3,9 @@
 //     o = softmax(s q1 k1^T) v - lambda softmax(s q2 k2^T) v,   out = (1 - lambda_init) RMS(o) w, or o.
 // One pass over the keys: each map keeps its running maximum, sum and product with V (the online
 // softmax), and the two are joined once both sums are known.
+//
+// Work of a pair (row, key) that a head sees: 4 hd operations for both maps' scores, 8 hd for their products with V (joined
+// before it the maps need 4 hd, but both sums first, so the scores twice: 12 hd as well), two exponentials. Long contexts are bound by these under the card's power limit, one new row by reading its cache.
 #include <math.h>
 
 #include <algorithm>
@@ -41,7 +44,8 @@ __device__ __forceinline__ float rms_factor(const DiffAttnArgs &a, float squares
     return squares == 0.0f ? 0.0f : (1.0f - a.lambda_init) / sqrtf(squares / (float)(2 * HD) + a.eps);
 }
 
-// Any stride and alignment: one wave a row and head. A block of 64 keys at a time, lane j takes the scores of key j;
+// Any stride and alignment (two samples of 397 rows, 8 heads, f16: 133 us; whole chunks 11): one wave a row and head. A
+// block of 64 keys at a time, lane j takes the scores of key j;
 // the probabilities go through LDS, then the lanes take the columns of V.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void diff_attn_any_kernel(const DiffAttnArgs a) {
@@ -495,6 +499,10 @@ __device__ __forceinline__ Part part_at(const DiffAttnArgs &a, const DiffPlan &p
     return p;
 }
 
+// Causal tiles are up to twice the mean length, and a CU's workgroups share it: started longest first, a CU gets two or
+// three of the longest and works on them when the others have ended. Lengths of 677 to 2047 rows, hd 32: 65.5 us in
+// the order of the static shapes, 51.2 as below; two samples of 8192 and 5620 rows, 2 heads of 4: 498, 325.
+//
 // Every other block of n workgroups of `all` turned round: n CUs get one of each block, the one with the longest tile of a
 // block the shortest of the next
 __device__ __forceinline__ int mirrored(int i, int n, int all) {
@@ -536,6 +544,10 @@ __device__ __forceinline__ bool ranked_part(const DiffAttnArgs &a, const DiffPla
 
 // A workgroup's worker: 128 rows, 32 a wave. The four waves share K and V tiles of 64 keys, two stages in LDS: the next is
 // loaded while one is worked on. Two workgroups a CU (hd 32: three), one's matrix products cover the other's softmax.
+// Measured: 12289 rows and keys, 8 heads, hd 64, f16: 938 us, 990 TFLOP/s of the 12 hd operations a pair (matrix units half
+// busy at 1.9 GHz, which the power limit leaves; a library bf16 product of 8192^3 reaches 1259). 1101 rows, 128 heads: 150
+// us, 790. One wave a SIMD, the products of a step beside the softmax of the one before: 1500 us for the first; 64 rows a
+// workgroup and two waves that share the keys: spills. Causal, hd 32, 677 to 2047 rows of four heads a key: 51 us.
 template <typename T, int HD>
 struct Wide {
     using L = Lay<HD>;
@@ -660,6 +672,9 @@ __device__ __forceinline__ float quad_sum(float v) {
     const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return pair_sum(__uint_as_float(p[0]) + __uint_as_float(p[1]));
 }
+// Measured: 64 caches of 2048 to 8192 keys, 4 heads of 4 rows, bf16: 121 us with the join, 5.8 TB/s of K and V (a large copy
+// on this card: 6.2); one row over 4099 keys, 8 heads: 12.2 us, 7.2 of it this kernel, all latency; two samples of 397
+// rows, 8 heads: 11 us (32 rows a workgroup that share their tiles: 13.1).
 template <typename T, int HD>
 struct Few {
     using L = Lay<HD>;
@@ -966,6 +981,8 @@ __global__ __launch_bounds__(256, A::WAVES) void diff_attn_kernel(const DiffAttn
 
 // Joins the pieces of the shared tiles, in the order of their keys: HD/2 lanes a row, four columns of each map a lane.
 // PG groups of lanes take a row's pieces in turn (as many as a workgroup has beside few rows) and are merged in LDS.
+// A launch of its own: 4 us behind one row over 4099 keys. The last workgroup of a tile joining it instead, by tickets,
+// takes device-wide fences that write back and drop an XCD's L2: 12.2 -> 15.3 us there, 140 -> 175 for 64 caches.
 template <typename T, int HD, int TR, int KB, int PG>
 __global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs a, const DiffPlan pl) {
     constexpr int LR = HD / 2, RPW = 256 / LR / PG;   // rows of a workgroup
@@ -1101,8 +1118,10 @@ struct DiffChoice {
 //  * wide tiles, a workgroup each: a unit takes 1.95 alone on a CU, 3.3 beside another
 //  * few-row tiles, a workgroup each: 0.95, 1.35
 //  * shared out: the same over 512 workgroups, and a second launch, and the pieces' way to memory and back
-// Measured, two samples of 8 heads, hd 64, full rows: 397 rows 11.7 few, 20.2 wide; 1101 rows 40.2, 39.7; 4096 rows 328,
-// 212. One row over 4099 keys, 8 heads: 33.7 a workgroup each, 12.2 shared; 64 sequences of 8192 keys: 200, 207.
+// Measured (us), two samples of 8 heads, hd 64, all keys: 397 rows 12 few, 20 wide; 1101 rows 41, 40; 4096 rows 328 few, 207
+// wide. One row over 4099 keys, 8 heads: 47 few-row tiles of a workgroup each, 12 shared out; 16 rows of four heads a key
+// over 2048 keys, 8 samples: 21, 24; 64 rows over 4096 keys, 4 samples of 8 heads: 37, 28. 64 caches of 8192 keys: 167,
+// 181, and with caches of 2048 to 8192 keys, as they are when lengths are given, 129, 121.
 DiffChoice choose(const DiffAttnArgs &a) {
     const long long rows = (long long)a.Sq * (a.nh / a.nkv), heads = (long long)a.nkv * a.B;
     const double h = a.hd == 64 ? 1.0 : 0.55;
@@ -1151,7 +1170,7 @@ DiffChoice choose(const DiffAttnArgs &a) {
                 const int shared = (int)std::min<long long>(wgs, units);
                 const double part = ceil((double)units / shared) * (wgs == 512 ? pair : alone) * ragged;
                 const double pieces = 2.0 * std::min<double>(shared + rest, units) * std::min<double>(tr, rows) * 16.25 * a.hd / 6e6;
-                keep(9 + n * (full / 512) * pair + std::max(part, stream * ragged) + pieces + (tr == 16 ? rest / 100.0 : 0.0), full, shared);
+                keep(10 + n * (full / 512) * pair + std::max(part, stream * ragged) + pieces + (tr == 16 ? rest / 40.0 : 0.0), full, shared);
             }
         }
     }
