@@ -454,7 +454,9 @@ def test_diff_attention(tsn, rt, dt, hd, B, Sq, Sk, nh, nkv, causal):
 # sizes at which the work is cut in each way, and the cuts fall inside tiles
 CUTS = [
     # B Sq Sk nh nkv causal kl heads
-    (130, 1, 4000, 2, 1, True, "ragged", None),        # one row of more than 64 samples: shared out by the lengths
+    (70, 1, 6000, 2, 1, True, "ragged", None),         # one row of more than 64 samples: shared out by the lengths
+    (66, 2, 6000, 2, 1, False, "some empty", None),
+    (130, 1, 4000, 2, 1, True, "ragged", None),        # a workgroup each
     (70, 3, 1500, 2, 1, False, "some empty", None),
     (1, 1, 70000, 2, 1, False, None, None),            # one row over a long cache
     (2, 40, 6000, 4, 1, True, "ragged", None),         # several tiles of few rows
@@ -467,6 +469,8 @@ CUTS = [
     (5, 1300, 1500, 40, 10, True, "ragged", (0, 23, 39)),      # causal tiles by length: all resident at once
     (33, 700, 700, 16, 8, True, "some empty", (0, 9, 15)),     # more of them, samples without rows and without keys
     (3, 1500, 400, 48, 48, True, "ragged", (0, 47)),           # more rows than keys: tiles without keys
+    (2, 4100, 4100, 12, 2, True, None, (0, 11)),               # heads that do not go round the XCDs
+    (70, 330, 330, 16, 8, True, "some empty", (0, 15)),        # more samples than are ranked
 ]
 
 
@@ -490,14 +494,15 @@ def test_diff_attention_cuts(tsn, rt, dt, hd, B, Sq, Sk, nh, nkv, causal, kl, he
     (3, 50, 90, 2, 1, True, [50, 50, 20], [10, 63, 90]),              # rows before the first key: empty
     (4, 1, 1500, 4, 2, True, [1, 1, 1, 1], [1500, 1, 0, 767]),
     (2, 1, 513, 8, 8, False, None, [512, 513]),
+    (3, 140, 210, 4, 2, True, [0, 139, 140], None),
     (3, 130, 260, 2, 2, False, [129, 130, 64], [65, 64, 1]),
     (2, 5, 3000, 2, 1, True, [5, 3], [2, 2999]),
     (2, 33, 128, 1, 1, False, [-5, 99], [200, -1]),                   # out of range: taken as none and all
 ])
 def test_diff_attention_lengths(tsn, rt, dt, junk, hd, B, Sq, Sk, nh, nkv, causal, ql, kl):
-    attn_case(tsn, rt, dt, B, Sq, Sk, nh, nkv, hd, causal, ql, [min(max(t, 0), Sk) for t in kl] if min(kl) < 0 or max(kl) > Sk else kl,
+    attn_case(tsn, rt, dt, B, Sq, Sk, nh, nkv, hd, causal, ql, [min(max(t, 0), Sk) for t in kl] if kl and (min(kl) < 0 or max(kl) > Sk) else kl,
               junk=junk)
-    if min(kl) < 0 or max(kl) > Sk:   # the same with the lengths as they are
+    if kl and (min(kl) < 0 or max(kl) > Sk):   # the same with the lengths as they are
         attn_case(tsn, rt, dt, B, Sq, Sk, nh, nkv, hd, causal, ql, kl)
 
 
