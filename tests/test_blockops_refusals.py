@@ -157,6 +157,10 @@ def test_wrappers_check_array_sizes(tsn):
         bad = dict(ok, **{k: Fake(ok[k].nbytes // 2 - 1, 2)})
         with pytest.raises(ValueError):
             rt.gate_add_norm(s, **bad)
+    gone = Fake(96, 4)   # a freed array is not an absent one
+    gone.p = None
+    with pytest.raises(ValueError, match="freed"):
+        rt.gate_add_norm(s, **dict(ok, post_w=gone))
     with pytest.raises(ValueError):
         tsn.rope_axes_spec(tsn.F32, 1, 1, 64, (8,) * 5, (1e4,) * 5)
     with pytest.raises(ValueError):

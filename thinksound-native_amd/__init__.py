@@ -142,7 +142,7 @@ class RopeAxesSpec(ctypes.Structure):
                 ("fscale", ctypes.c_float * 4), ("half_split", ctypes.c_int), ("inverse", ctypes.c_int)]
 
     def sizes(self):
-        """(array, bytes, optional) of x, pos, y"""
+        """(array, bytes, optional) in the order of tsn_rope_axes"""
         n, size = self.nh * self.hd, 4 if self.dtype == F32 else 2
         return (("x", _span(self.rows, self.ldx or n, n) * size, False),
                 ("pos", (self.pos_rows or self.rows) * self.n_axes * 4, False),
@@ -159,12 +159,13 @@ class DiffAttnSpec(ctypes.Structure):
                 ("lambda_init", ctypes.c_float), ("eps", ctypes.c_float)]
 
     def sizes(self):
-        """(array, bytes, optional) of q, k, v, out, lam, norm_w, q_len, kv_len"""
+        """(array, bytes, optional) in the order of tsn_diff_attention"""
         B, Sq, Sk, hd = self.B, self.Sq, self.Sk, self.hd
         wq, wk = 2 * self.nh * hd, 2 * self.nkv * hd
         return (("q", 2 * _span3(B, Sq, self.ldq or wq, self.bsq, wq), False), ("k", 2 * _span3(B, Sk, self.ldk or wk, self.bsk, wk), False),
-                ("v", 2 * _span3(B, Sk, self.ldv or wk, self.bsv, wk), False), ("out", 2 * _span3(B, Sq, self.ldo or wq, self.bso, wq), False),
-                ("lam", 16 * self.lam_heads * hd, False), ("norm_w", 8 * hd, True), ("q_len", 4 * B, True), ("kv_len", 4 * B, True))
+                ("v", 2 * _span3(B, Sk, self.ldv or wk, self.bsv, wk), False), ("lam", 16 * self.lam_heads * hd, False),
+                ("norm_w", 8 * hd, True), ("q_len", 4 * B, True), ("kv_len", 4 * B, True),
+                ("out", 2 * _span3(B, Sq, self.ldo or wq, self.bso, wq), False))
 
 
 class GateNormSpec(ctypes.Structure):
@@ -177,13 +178,13 @@ class GateNormSpec(ctypes.Structure):
                 ("post_eps", ctypes.c_float), ("pre_eps", ctypes.c_float)]
 
     def sizes(self):
-        """(array, bytes, optional) of x, f, x_out, y, mod, post_w, post_b, pre_w, pre_b"""
+        """(array, bytes, optional) in the order of tsn_gate_add_norm"""
         rows, H, m = self.rows, self.H, self.mod_rows
         sx, sf, sy = (4 if dt == F32 else 2 for dt in (self.x_dtype, self.f_dtype, self.y_dtype))
         return (("x", _span(rows, self.ldx or H, H) * sx, False), ("f", _span(rows, self.ldf or H, H) * sf, False),
-                ("x_out", _span(rows, self.ldo or H, H) * sx, False), ("y", _span(rows, self.ldy or H, H) * sy, True),
                 ("mod", (-(-rows // m) if m else 1) * self.chunks * H * 4, True), ("post_w", 4 * H, True),
-                ("post_b", 4 * H, True), ("pre_w", 4 * H, True), ("pre_b", 4 * H, True))
+                ("post_b", 4 * H, True), ("pre_w", 4 * H, True), ("pre_b", 4 * H, True),
+                ("x_out", _span(rows, self.ldo or H, H) * sx, False), ("y", _span(rows, self.ldy or H, H) * sy, True))
 
 
 class KernelStat(ctypes.Structure):
@@ -1018,19 +1019,16 @@ class Runtime:
     # --- block operators: device arrays, and a spec made once (rope_axes_spec, diff_attn_spec, gate_norm_spec) ---
     def rope_axes(self, spec, x, pos, y):
         """multi-axis rotary positions of the heads in x's rows, to y (which may be x)"""
-        _hold("rope_axes", spec, (x, pos, y))
-        call("tsn_rope_axes", self.h, spec, x.p, pos.p, y.p)
+        call("tsn_rope_axes", self.h, spec, *_hold("rope_axes", spec, (x, pos, y)))
 
     def diff_attention(self, spec, q, k, v, lam, norm_w, q_len, kv_len, out):
         """differential attention; norm_w, q_len and kv_len may be None"""
-        _hold("diff_attention", spec, (q, k, v, out, lam, norm_w, q_len, kv_len))
-        call("tsn_diff_attention", self.h, spec, q.p, k.p, v.p, lam.p, _p(norm_w), _p(q_len), _p(kv_len), out.p)
+        call("tsn_diff_attention", self.h, spec, *_hold("diff_attention", spec, (q, k, v, lam, norm_w, q_len, kv_len, out)))
 
     def gate_add_norm(self, spec, x, f, mod, x_out, y, post_w=None, post_b=None, pre_w=None, pre_b=None):
         """x_out = x_scale*x + f_scale*gate*post(f), y = pre(x_out)*(1 + scale) + shift; y and mod may be None"""
-        _hold("gate_add_norm", spec, (x, f, x_out, y, mod, post_w, post_b, pre_w, pre_b))
-        call("tsn_gate_add_norm", self.h, spec, x.p, f.p, _p(mod), _p(post_w), _p(post_b), _p(pre_w), _p(pre_b), x_out.p,
-             _p(y))
+        call("tsn_gate_add_norm", self.h, spec,
+             *_hold("gate_add_norm", spec, (x, f, mod, post_w, post_b, pre_w, pre_b, x_out, y)))
 
     def silu(self, x, n):
         call("tsn_silu", self.h, x.p, n)
@@ -1072,21 +1070,20 @@ def _need(what, arr, numel, itemsize=4, optional=False):
 
 
 def _hold(what, spec, arrays):
-    """_need of a block operator's arrays, in the order of the spec's sizes(); the spec keeps them until a field changes"""
+    """_need of a block operator's arrays, in the order of the spec's sizes(), which the spec keeps until a field changes;
+    their device pointers"""
     key = bytes(spec)
     kept = spec.__dict__.get("_kept")
     if kept is None or kept[0] != key:
         kept = spec._kept = key, spec.sizes()
-    for arr, size in zip(arrays, kept[1]):
-        if arr is None:
-            if not size[2]:
-                raise ValueError("%s: %s: a device array is required" % (what, size[0]))
-        elif arr.__class__ is not DeviceArray and not hasattr(arr, "p") or arr.nbytes < size[1]:
-            _need("%s: %s" % (what, size[0]), arr, size[1], 1)
-
-
-def _p(arr):
-    return None if arr is None else arr.p
+    ptrs = [getattr(arr, "p", None) for arr in arrays]
+    for arr, p, (name, size, optional) in zip(arrays, ptrs, kept[1]):
+        if arr is None and optional:
+            continue
+        if p is None or arr.nbytes < size:
+            _need("%s: %s" % (what, name), arr, size, 1)
+            raise ValueError("%s: %s: the array has been freed" % (what, name))
+    return ptrs
 
 
 def _span(rows, ld, width):

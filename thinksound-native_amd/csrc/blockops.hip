@@ -461,11 +461,18 @@ RopeKernelArgs<NP> rope_kernel_args(const RopeAxesArgs &c) {
     for (unsigned i = 0; i < c.n_axes; ++i) {
         a.start[i] = a.total;
         a.dim[i] = c.dim[i];
-        // pair by pair times base^(-2/dim), in 64 bits of mantissa: 128 roundings are 2^-57, a pow a pair 1 us a call more
-        const long double ratio = c.dim[i] ? powl((long double)c.base[i], -2.0L / c.dim[i]) : 1.0L;
-        long double f = (c.inverse ? -1.0L : 1.0L) * c.fscale[i] / (2.0L * 3.14159265358979323846264338327950288L);
-        for (unsigned p = 0; p < c.dim[i] / 2; ++p, f *= ratio) a.freq[a.total / 2 + p] = (double)f;
         a.total += c.dim[i];
+        const unsigned n = c.dim[i] / 2;
+        if (n == 0) continue;
+        // Pair by pair times base^(-1/n), in 64 bits of mantissa: n roundings are 2^-57 at most. The factor is that of pow
+        // with one step of Newton's for factor^n base = 1. (A pow for each pair takes 1.5 us a call more, powl 0.7.)
+        const double near = pow((double)c.base[i], -1.0 / n);
+        long double q = c.base[i], power = near;
+        for (unsigned e = n; e; e >>= 1, power *= power)
+            if (e & 1) q *= power;
+        const long double ratio = near + near * ((1.0L - q) / n);
+        long double f = (c.inverse ? -1.0L : 1.0L) * c.fscale[i] / (2.0L * 3.14159265358979323846264338327950288L);
+        for (unsigned p = 0; p < n; ++p, f *= ratio) a.freq[a.start[i] / 2 + p] = (double)f;
     }
     return a;
 }
