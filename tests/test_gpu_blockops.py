@@ -94,6 +94,10 @@ ROPES = [
     (F32, 33, 3, 80, (8, 24, 16), True, False, 0, 0, 0, 11),
     (F16, 41, 3, 80, (8, 24, 16), False, True, 0, 0, 0, 0),
     (F16, 17, 3, 80, (12, 28, 20), True, False, 0, 0, 0, 0),         # halves that are no multiple of 8
+    (F16, 65, 16, 64, (16, 24, 24), True, False, 0, 0, 0, 13),       # halves of 12: chunks of 8 bytes
+    (BF16, 37, 5, 60, (24, 24), True, True, 308, 0, 4, 0),           # rows aligned to 8 bytes
+    (F16, 1000, 3, 200, (40, 56, 72), True, False, 0, 604, 0, 0),
+    (BF16, 37, 5, 60, (24, 24), True, True, 310, 0, 2, 0),           # and to 4: one element at a time
     (F16, 29, 7, 64, (16, 24, 24), False, False, 1344, 0, 448, 0),   # k heads out of q|k|v rows
     (F16, 29, 7, 64, (16, 24, 24), False, False, 451, 449, 1, 0),    # odd strides
     (BF16, 19, 3, 70, (10, 20, 30, 4), False, False, 0, 0, 0, 0),    # a width that is no multiple of 8, four axes
@@ -146,11 +150,12 @@ def spread(n, r):
     return np.unique(np.concatenate([np.arange(40), r.integers(0, n, 400), np.arange(n - 40, n)]))
 
 
-@pytest.mark.parametrize("dt,half", [(F32, False), (F16, True), (F16, False), (BF16, True)])
-def test_rope_axes_large(tsn, rt, dt, half):
+@pytest.mark.parametrize("dt,half,dims", [(F32, False, (16, 16, 32)), (F16, True, (16, 16, 32)), (F16, False, (16, 16, 32)),
+                                          (BF16, True, (16, 16, 32)), (F16, True, (16, 24, 24))])
+def test_rope_axes_large(tsn, rt, dt, half, dims):
     """traffic past the last-level cache (over 192 MiB), an odd number of rows"""
     r = rng(12)
-    nh, hd, dims, bases = 32, 64, (16, 16, 32), (1e4, 1e2, 1e2)
+    nh, hd, bases = 32, 64, (1e4, 1e2, 1e2)
     rows = (13 if dt == F32 else 26) * 1000 + 1
     some = enc(r.standard_normal((997, nh * hd)), dt)
     x = some[np.arange(rows) % 997]

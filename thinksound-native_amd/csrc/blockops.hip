@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256) void rope_axes_any_kernel(const RopeKernelArgs
     }
 }
 
-// Whole 16-byte chunks: a workgroup takes rb rows, computes the cosines and sines of their pairs once (in LDS, for all
+// Whole chunks of VE elements (16 bytes; 8 where halves of 16-bit axes do not divide into more): a workgroup takes rb rows, computes the cosines and sines of their pairs once (in LDS, for all
 // heads) while its first chunks are under way, and turns them. An item is a chunk (neighbouring pairs) or the two
 // chunks that hold a pair's halves; behind the axes a chunk is copied. per_head items a head, per_row a row;
 // the magic numbers divide by them.
@@ -90,9 +90,9 @@ __global__ __launch_bounds__(256) void rope_axes_any_kernel(const RopeKernelArgs
 struct RopeChunks {
     unsigned rb, per_head, per_row, head_magic, row_magic;
 };
-template <typename T, bool HALF, bool ONCE, int NP>
+template <typename T, bool HALF, bool ONCE, int NP, int VE>
 __global__ __launch_bounds__(256) void rope_axes_kernel(const RopeKernelArgs<NP> a, const RopeChunks c) {
-    constexpr int VE = 16 / sizeof(T), UN = 4;   // elements of a chunk; items in flight a thread
+    constexpr int UN = 4;   // items in flight a thread
     typedef T vec __attribute__((ext_vector_type(VE)));
     extern __shared__ float2 table[];   // [row of the workgroup][pair]
     const unsigned np = a.hd / 2, r0 = blockIdx.x * c.rb, rows = min(c.rb, a.rows - r0), items = rows * c.per_row;
@@ -477,39 +477,42 @@ RopeKernelArgs<NP> rope_kernel_args(const RopeAxesArgs &c) {
     return a;
 }
 
-template <typename T, int NP>
+template <typename T, int NP, int VE>
 int launch_rope_chunks(const RopeAxesArgs &c, const RopeChunks &k, hipStream_t st) {
     const RopeKernelArgs<NP> a = rope_kernel_args<NP>(c);
     const dim3 grid((c.rows + k.rb - 1) / k.rb);
     const size_t lds = (size_t)k.rb * (c.hd / 2) * sizeof(float2);
     const bool once = passes_caches((size_t)2 * c.rows * c.nh * c.hd * sizeof(T));
     if (c.half_split) {
-        if (once) TSN_LAUNCH((rope_axes_kernel<T, true, true, NP>), grid, dim3(256), lds, st, a, k);
-        else TSN_LAUNCH((rope_axes_kernel<T, true, false, NP>), grid, dim3(256), lds, st, a, k);
-    } else {
-        if (once) TSN_LAUNCH((rope_axes_kernel<T, false, true, NP>), grid, dim3(256), lds, st, a, k);
-        else TSN_LAUNCH((rope_axes_kernel<T, false, false, NP>), grid, dim3(256), lds, st, a, k);
+        if (once) TSN_LAUNCH((rope_axes_kernel<T, true, true, NP, VE>), grid, dim3(256), lds, st, a, k);
+        else TSN_LAUNCH((rope_axes_kernel<T, true, false, NP, VE>), grid, dim3(256), lds, st, a, k);
+    } else if constexpr (VE * sizeof(T) == 16) {
+        if (once) TSN_LAUNCH((rope_axes_kernel<T, false, true, NP, VE>), grid, dim3(256), lds, st, a, k);
+        else TSN_LAUNCH((rope_axes_kernel<T, false, false, NP, VE>), grid, dim3(256), lds, st, a, k);
     }
     TSN_HIP_CHECK(hipGetLastError());
     return TSN_OK;
 }
-template <typename T>
+template <typename T, int VE>
 int launch_rope_typed(const RopeAxesArgs &c, const RopeChunks &k, hipStream_t st) {
-    return c.hd <= 64 ? launch_rope_chunks<T, 32>(c, k, st) : launch_rope_chunks<T, MAX_PAIRS>(c, k, st);
+    return c.hd <= 64 ? launch_rope_chunks<T, 32, VE>(c, k, st) : launch_rope_chunks<T, MAX_PAIRS, VE>(c, k, st);
 }
 
 } // namespace
 
 int launch_rope_axes(const RopeAxesArgs &c, hipStream_t st) {
-    // whole chunks: aligned rows and heads, and for halves whole chunks of each half
-    const unsigned ve = c.dt == DT_F32 ? 4 : 8;
-    unsigned total = 0;
-    bool whole = (((uintptr_t)c.x | (uintptr_t)c.y) & 15) == 0 && c.ldx % ve == 0 && c.ldy % ve == 0 && c.hd % ve == 0;
+    unsigned total = 0, halves = 0;
     for (unsigned i = 0; i < c.n_axes; ++i) {
-        whole = whole && (!c.half_split || c.dim[i] % (2 * ve) == 0);
         total += c.dim[i];
+        halves |= c.dim[i] / 2;
     }
-    if (whole) {
+    // whole chunks: aligned rows and heads, and for halves whole chunks of each half
+    auto whole = [&](unsigned ve) {
+        const unsigned at = (unsigned)((uintptr_t)c.x | (uintptr_t)c.y) / (unsigned)elem_bytes(c.dt);
+        return ((at | c.ldx | c.ldy | c.hd | (c.half_split ? halves : 0)) & (ve - 1)) == 0;
+    };
+    const unsigned ve = c.half_split && c.dt != DT_F32 && !whole(8) ? 4 : c.dt == DT_F32 ? 4 : 8;
+    if (whole(ve)) {
         RopeChunks k{};
         k.per_head = c.half_split ? (total / 2 + (c.hd - total)) / ve : c.hd / ve;
         k.per_row = c.nh * k.per_head;
@@ -523,8 +526,9 @@ int launch_rope_axes(const RopeAxesArgs &c, hipStream_t st) {
         k.row_magic = magic(k.per_row);
         const unsigned long long most = (unsigned long long)k.rb * k.per_row;
         if (k.per_head > 1 && most * k.per_row < (1ULL << 32) && k.rb <= 16384 / c.hd) {
-            if (c.dt == DT_F32) return launch_rope_typed<float>(c, k, st);
-            return c.dt == DT_F16 ? launch_rope_typed<half_t>(c, k, st) : launch_rope_typed<bf16_t>(c, k, st);
+            if (c.dt == DT_F32) return launch_rope_typed<float, 4>(c, k, st);
+            if (ve == 4) return c.dt == DT_F16 ? launch_rope_typed<half_t, 4>(c, k, st) : launch_rope_typed<bf16_t, 4>(c, k, st);
+            return c.dt == DT_F16 ? launch_rope_typed<half_t, 8>(c, k, st) : launch_rope_typed<bf16_t, 8>(c, k, st);
         }
     }
     const RopeKernelArgs<MAX_PAIRS> a = rope_kernel_args<MAX_PAIRS>(c);
