@@ -501,13 +501,13 @@ __device__ __forceinline__ Part part_at(const DiffAttnArgs &a, const DiffPlan &p
 
 // Causal tiles are up to twice the mean length, and a CU's workgroups share it: started longest first, a CU gets two or
 // three of the longest and works on them when the others have ended. Lengths of 677 to 2047 rows, hd 32: 65.5 us in
-// the order of the static shapes, 51.2 as below; two samples of 8192 and 5620 rows, 2 heads of 4: 498, 325.
+// the order of the static shapes, 51 as below; two samples of 8192 and 5620 rows, 2 heads of 4: 498, 325.
 //
-// Every other block of n workgroups of `all` turned round: n CUs get one of each block, the one with the longest tile of a
-// block the shortest of the next
+// Blocks of n workgroups of `all` behind the first turned round: n CUs get one of each block, the one with the longest of
+// the first the shortest of the others (every other block turned round: 2% slower)
 __device__ __forceinline__ int mirrored(int i, int n, int all) {
     const int block = i / n, first = block * n;
-    return block & 1 ? first + min(n, all - first) - 1 - (i - first) : i;
+    return block ? first + min(n, all - first) - 1 - (i - first) : i;
 }
 // Causal tiles of up to 64 samples of unequal length, longest first over all: a sample's tiles end at level
 // nk*G/TR, one level apart. Sets b, nq, nk, g, tile and returns whether there is a tile of the workgroup's rank. Samples
@@ -547,7 +547,7 @@ __device__ __forceinline__ bool ranked_part(const DiffAttnArgs &a, const DiffPla
 // Measured: 12289 rows and keys, 8 heads, hd 64, f16: 938 us, 990 TFLOP/s of the 12 hd operations a pair (matrix units half
 // busy at 1.9 GHz, which the power limit leaves; a library bf16 product of 8192^3 reaches 1259). 1101 rows, 128 heads: 150
 // us, 790. One wave a SIMD, the products of a step beside the softmax of the one before: 1500 us for the first; 64 rows a
-// workgroup and two waves that share the keys: spills. Causal, hd 32, 677 to 2047 rows of four heads a key: 51 us.
+// workgroup and two waves that share the keys: spills. Causal, hd 32, 677 to 2047 rows of four heads a key: 48.6 us.
 template <typename T, int HD>
 struct Wide {
     using L = Lay<HD>;
@@ -593,7 +593,7 @@ struct Wide {
             block_barrier();
             if (u + 1 < end) issue(u + 1);
             const unsigned at = (u & 1) * STAGE;
-#pragma unroll 1
+#pragma unroll   // one block's start beside the other's end: hd 32, as above, 51.1 -> 48.6 us; hd 64 1 to 4%
             for (int i = 0; i < KB / 32; ++i) {
                 const int k0 = u * KB + 32 * i;
                 floatx16 s[2];
