@@ -97,7 +97,10 @@ ROPES = [
     (F16, 65, 16, 64, (16, 24, 24), True, False, 0, 0, 0, 13),       # halves of 12: chunks of 8 bytes
     (BF16, 37, 5, 60, (24, 24), True, True, 308, 0, 4, 0),           # rows aligned to 8 bytes
     (F16, 1000, 3, 200, (40, 56, 72), True, False, 0, 604, 0, 0),
-    (BF16, 37, 5, 60, (24, 24), True, True, 310, 0, 2, 0),           # and to 4: one element at a time
+    (BF16, 37, 5, 60, (24, 24), True, True, 310, 0, 2, 0),           # and to 4
+    (F32, 65, 6, 80, (4, 12, 20), True, False, 0, 504, 0, 13),       # halves of 2, 6 and 10
+    (F16, 300, 20, 128, (4, 28, 60), True, False, 0, 0, 0, 100),
+    (BF16, 37, 5, 58, (4, 24), True, True, 299, 0, 3, 0),            # one element at a time
     (F16, 29, 7, 64, (16, 24, 24), False, False, 1344, 0, 448, 0),   # k heads out of q|k|v rows
     (F16, 29, 7, 64, (16, 24, 24), False, False, 451, 449, 1, 0),    # odd strides
     (BF16, 19, 3, 70, (10, 20, 30, 4), False, False, 0, 0, 0, 0),    # a width that is no multiple of 8, four axes

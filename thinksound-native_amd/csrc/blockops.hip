@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256) void rope_axes_any_kernel(const RopeKernelArgs
     }
 }
 
-// Whole chunks of VE elements (16 bytes; 8 where halves of 16-bit axes do not divide into more): a workgroup takes rb rows, computes the cosines and sines of their pairs once (in LDS, for all
+// Whole chunks of VE elements (16 bytes; 8 or two elements where halves of axes do not divide into more): a workgroup takes rb rows, computes the cosines and sines of their pairs once (in LDS, for all
 // heads) while its first chunks are under way, and turns them. An item is a chunk (neighbouring pairs) or the two
 // chunks that hold a pair's halves; behind the axes a chunk is copied. per_head items a head, per_row a row;
 // the magic numbers divide by them.
@@ -486,7 +486,7 @@ int launch_rope_chunks(const RopeAxesArgs &c, const RopeChunks &k, hipStream_t s
     if (c.half_split) {
         if (once) TSN_LAUNCH((rope_axes_kernel<T, true, true, NP, VE>), grid, dim3(256), lds, st, a, k);
         else TSN_LAUNCH((rope_axes_kernel<T, true, false, NP, VE>), grid, dim3(256), lds, st, a, k);
-    } else if constexpr (VE * sizeof(T) == 16) {
+    } else if constexpr (VE * sizeof(T) == 16) {   // neighbours: whole chunks whatever the axes are
         if (once) TSN_LAUNCH((rope_axes_kernel<T, false, true, NP, VE>), grid, dim3(256), lds, st, a, k);
         else TSN_LAUNCH((rope_axes_kernel<T, false, false, NP, VE>), grid, dim3(256), lds, st, a, k);
     }
@@ -511,7 +511,8 @@ int launch_rope_axes(const RopeAxesArgs &c, hipStream_t st) {
         const unsigned at = (unsigned)((uintptr_t)c.x | (uintptr_t)c.y) / (unsigned)elem_bytes(c.dt);
         return ((at | c.ldx | c.ldy | c.hd | (c.half_split ? halves : 0)) & (ve - 1)) == 0;
     };
-    const unsigned ve = c.half_split && c.dt != DT_F32 && !whole(8) ? 4 : c.dt == DT_F32 ? 4 : 8;
+    unsigned ve = c.dt == DT_F32 ? 4 : 8;
+    while (c.half_split && ve > 2 && !whole(ve)) ve /= 2;
     if (whole(ve)) {
         RopeChunks k{};
         k.per_head = c.half_split ? (total / 2 + (c.hd - total)) / ve : c.hd / ve;
@@ -526,7 +527,8 @@ int launch_rope_axes(const RopeAxesArgs &c, hipStream_t st) {
         k.row_magic = magic(k.per_row);
         const unsigned long long most = (unsigned long long)k.rb * k.per_row;
         if (k.per_head > 1 && most * k.per_row < (1ULL << 32) && k.rb <= 16384 / c.hd) {
-            if (c.dt == DT_F32) return launch_rope_typed<float, 4>(c, k, st);
+            if (c.dt == DT_F32) return ve == 4 ? launch_rope_typed<float, 4>(c, k, st) : launch_rope_typed<float, 2>(c, k, st);
+            if (ve == 2) return c.dt == DT_F16 ? launch_rope_typed<half_t, 2>(c, k, st) : launch_rope_typed<bf16_t, 2>(c, k, st);
             if (ve == 4) return c.dt == DT_F16 ? launch_rope_typed<half_t, 4>(c, k, st) : launch_rope_typed<bf16_t, 4>(c, k, st);
             return c.dt == DT_F16 ? launch_rope_typed<half_t, 8>(c, k, st) : launch_rope_typed<bf16_t, 8>(c, k, st);
         }
