@@ -278,13 +278,62 @@ __global__ __launch_bounds__(256) void gate_norm_any_kernel(const GateNormArgs a
 // f_scale gate post_b, made anew where a row of mod begins.
 // Bound by memory: 32771 rows of 2048, bf16, each with its row of mod (1.34 GB): 227 us, 5.9 TB/s (a large copy: 6.2); 6352
 // rows of 1024 with shared modulation, f32 and f16: 15.7 us, 5.0 TB/s; 8 rows: 3.5 us, a launch and a chain of four sums.
-template <typename TX, typename TF, int W, int NC, bool ONCE>
+// ANY: rows of any alignment and width: a lane's elements are 64 W apart, loaded and stored one by one, so that a wave's
+// access is of neighbours wherever a row begins (16-byte accesses at odd places: 20000 rows of 2501, bf16, each with its
+// row of mod XX -> 440 us; a row in LDS 379).
+template <typename TX, typename TF, int W, int NC, bool ONCE, bool ANY>
 __global__ __launch_bounds__(W > 1 ? 64 * W : 256, NC == 1 ? 4 : 2) void gate_norm_kernel(const GateNormArgs a, unsigned per) {
     constexpr int GROUPS = W > 1 ? 1 : 4;   // row groups of a workgroup
     __shared__ float red_all[GROUPS][W];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     float *red = red_all[wave / W];
     const unsigned H = a.H, chunks = H / 8, first = (wave % W) * 64 + lane;
+    // chunk c of the lane: elements 8 k on, k = 64 W c + first, or (ANY) 64 W (8 c + e) + first, e = 0..7
+    auto there = [&](int c) { return ANY || c * 64 * W + first < chunks; };
+    auto place = [&](int c, int e) { return (8 * c + e) * 64 * W + first; };
+    // ANY: a row as a buffer of its own, whose elements from H on read as zeros and are not written
+    auto buffer = [&](auto *p) { return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, (int)(H * sizeof(*p)), 0x00020000); };
+    auto load8 = [&](auto *p, int c) {
+        typedef std::remove_cv_t<std::remove_pointer_t<decltype(p)>> T;
+        typedef typename Eight<T>::type V;
+        if constexpr (ANY) {
+            const auto row = buffer(p);
+            V v;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int lane_at = first * sizeof(T), at = (8 * c + e) * 64 * W * sizeof(T);
+                if constexpr (sizeof(T) == 4) v[e] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(row, lane_at, at, 0));
+                else v[e] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(row, lane_at, at, 0));
+            }
+            return v;
+        } else {
+            return *(const V *)(p + 8 * (c * 64 * W + first));
+        }
+    };
+    auto put8 = [&](auto *p, int c, const floatx8 &v) {
+        typedef std::remove_pointer_t<decltype(p)> T;
+        if constexpr (ANY) {
+            const auto row = buffer(p);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int lane_at = first * sizeof(T), at = (8 * c + e) * 64 * W * sizeof(T);
+                if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint((float)v[e]), row, lane_at, at, 0);
+                else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (T)v[e]), row, lane_at, at, 0);
+            }
+        } else {
+            store8(p + 8 * (c * 64 * W + first), v, std::integral_constant<bool, ONCE>());
+        }
+    };
+    // zeros where there is no element
+    auto clear = [&](floatx8 &v, int c) {
+        if constexpr (ANY) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (place(c, e) >= H) v[e] = 0.0f;
+        } else {
+            if (!there(c)) v = floatx8{};
+        }
+    };
     const unsigned group = blockIdx.x * GROUPS + wave / W;
     const unsigned r0 = group * per, r1 = min(r0 + per, a.rows);
     const float n = (float)H;
@@ -313,8 +362,10 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256, NC == 1 ? 4 : 2) void gate_no
             for (int c = 0; c < NC; ++c) s += sum8(x[c]);
             const float mean = row_sum(s) / n;
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
-                if (c * 64 * W + first < chunks) x[c] -= mean;
+            for (int c = 0; c < NC; ++c) {
+                x[c] -= mean;
+                clear(x[c], c);
+            }
             s = 0.0f;
         }
 #pragma unroll
@@ -326,10 +377,9 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256, NC == 1 ? 4 : 2) void gate_no
     auto load = [&](unsigned r) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const unsigned k = c * 64 * W + first;
-            if (k < chunks) {
-                rf[c] = *(const typename Eight<TF>::type *)((const TF *)a.f + (unsigned long long)r * a.ldf + 8 * k);
-                rx[c] = *(const typename Eight<TX>::type *)((const TX *)a.x + (unsigned long long)r * a.ldx + 8 * k);
+            if (there(c)) {
+                rf[c] = load8((const TF *)a.f + (unsigned long long)r * a.ldf, c);
+                rx[c] = load8((const TX *)a.x + (unsigned long long)r * a.ldx, c);
             } else {
                 rf[c] = typename Eight<TF>::type{};
                 rx[c] = typename Eight<TX>::type{};
@@ -345,9 +395,9 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256, NC == 1 ? 4 : 2) void gate_no
             const float *mod = a.mod ? a.mod + (unsigned long long)m * a.chunks * H : nullptr;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const unsigned k = min(c * 64 * W + first, chunks - 1);
+                const floatx8 none{};
                 auto vec = [&](const float *p, float other) {
-                    return p ? *(const floatx8 *)(p + 8 * k) : floatx8{other, other, other, other, other, other, other, other};
+                    return !p ? none + other : there(c) ? load8(p, c) : none;
                 };
                 const floatx8 g = vec(a.gate >= 0 ? mod + (unsigned long long)a.gate * H : nullptr, 1.0f) * a.f_scale;
                 const floatx8 s = 1.0f + vec(a.scale >= 0 ? mod + (unsigned long long)a.scale * H : nullptr, 0.0f);
@@ -366,27 +416,25 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256, NC == 1 ? 4 : 2) void gate_no
         const float inv = norm(f, a.post, a.post_eps);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const unsigned k = c * 64 * W + first;
             x[c] += f[c] * inv * G[c] + D[c];
-            if (k < chunks) store8((TX *)a.x_out + (unsigned long long)r * a.ldo + 8 * k, x[c], std::integral_constant<bool, ONCE>());
-            else x[c] = floatx8{};
+            if (there(c)) put8((TX *)a.x_out + (unsigned long long)r * a.ldo, c, x[c]);
+            clear(x[c], c);
         }
         if (!a.y) continue;
         const float pinv = norm(x, a.pre, a.pre_eps);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const unsigned k = c * 64 * W + first;
-            if (k >= chunks) break;
+            if (!there(c)) break;
             const floatx8 y = x[c] * pinv * A[c] + B[c];
-            const unsigned long long at = (unsigned long long)r * a.ldy + 8 * k;
-            if (a.ydt == DT_F32) store8((float *)a.y + at, y, std::integral_constant<bool, ONCE>());
-            else if (a.ydt == DT_F16) store8((half_t *)a.y + at, y, std::integral_constant<bool, ONCE>());
-            else store8((bf16_t *)a.y + at, y, std::integral_constant<bool, ONCE>());
+            const unsigned long long at = (unsigned long long)r * a.ldy;
+            if (a.ydt == DT_F32) put8((float *)a.y + at, c, y);
+            else if (a.ydt == DT_F16) put8((half_t *)a.y + at, c, y);
+            else put8((bf16_t *)a.y + at, c, y);
         }
     }
 }
 
-template <typename TX, typename TF, int W, int NC>
+template <typename TX, typename TF, int W, int NC, bool ANY>
 int launch_gate_norm_rows(const GateNormArgs &a, hipStream_t st) {
     constexpr unsigned GROUPS = W > 1 ? 1 : 4;
     // Rows that share a row of mod in turn, so that the waves fill the device once (16 or 8 a CU): 6352 rows of 1024 take
@@ -397,25 +445,31 @@ int launch_gate_norm_rows(const GateNormArgs &a, hipStream_t st) {
     const unsigned per = std::max(a.mod_rows == 1 ? 1u : std::min(waves, 32u), (a.rows >> 22) + 1);   // a launch has less than 2^32 threads
     const unsigned groups = a.rows / per + (a.rows % per != 0);
     const dim3 grid((groups + GROUPS - 1) / GROUPS), block(W > 1 ? 64 * W : 256);
-    if (passes_caches((size_t)a.rows * a.H * (2 * sizeof(TX) + sizeof(TF) + (a.y ? elem_bytes(a.ydt) : 0))))
-        TSN_LAUNCH((gate_norm_kernel<TX, TF, W, NC, true>), grid, block, 0, st, a, per);
-    else
-        TSN_LAUNCH((gate_norm_kernel<TX, TF, W, NC, false>), grid, block, 0, st, a, per);
+    const bool once = passes_caches((size_t)a.rows * a.H * (2 * sizeof(TX) + sizeof(TF) + (a.y ? elem_bytes(a.ydt) : 0)));
+    if constexpr (ANY) TSN_LAUNCH((gate_norm_kernel<TX, TF, W, NC, false, true>), grid, block, 0, st, a, per);
+    else if (once) TSN_LAUNCH((gate_norm_kernel<TX, TF, W, NC, true, false>), grid, block, 0, st, a, per);
+    else TSN_LAUNCH((gate_norm_kernel<TX, TF, W, NC, false, false>), grid, block, 0, st, a, per);
     TSN_HIP_CHECK(hipGetLastError());
     return TSN_OK;
 }
 template <typename TX, typename TF>
-int launch_gate_norm_typed(const GateNormArgs &a, hipStream_t st) {
-    if (a.H <= 512) return launch_gate_norm_rows<TX, TF, 1, 1>(a, st);
-    if (a.H <= 1024) return launch_gate_norm_rows<TX, TF, 2, 1>(a, st);
-    if (a.H <= 2048) return launch_gate_norm_rows<TX, TF, 2, 2>(a, st);
-    if (a.H <= 4096) return launch_gate_norm_rows<TX, TF, 4, 2>(a, st);
-    return launch_gate_norm_rows<TX, TF, 8, 2>(a, st);   // to 8192
+int launch_gate_norm_typed(const GateNormArgs &a, bool aligned, hipStream_t st) {
+    if (!aligned) {   // to 4096; two chunks a lane would spill their addresses
+        if (a.H <= 512) return launch_gate_norm_rows<TX, TF, 1, 1, true>(a, st);
+        if (a.H <= 1024) return launch_gate_norm_rows<TX, TF, 2, 1, true>(a, st);
+        if (a.H <= 2048) return launch_gate_norm_rows<TX, TF, 4, 1, true>(a, st);
+        return launch_gate_norm_rows<TX, TF, 8, 1, true>(a, st);
+    }
+    if (a.H <= 512) return launch_gate_norm_rows<TX, TF, 1, 1, false>(a, st);
+    if (a.H <= 1024) return launch_gate_norm_rows<TX, TF, 2, 1, false>(a, st);
+    if (a.H <= 2048) return launch_gate_norm_rows<TX, TF, 2, 2, false>(a, st);
+    if (a.H <= 4096) return launch_gate_norm_rows<TX, TF, 4, 2, false>(a, st);
+    return launch_gate_norm_rows<TX, TF, 8, 2, false>(a, st);   // to 8192
 }
 template <typename TX>
-int launch_gate_norm_f(const GateNormArgs &a, hipStream_t st) {
-    if (a.fdt == DT_F32) return launch_gate_norm_typed<TX, float>(a, st);
-    return a.fdt == DT_F16 ? launch_gate_norm_typed<TX, half_t>(a, st) : launch_gate_norm_typed<TX, bf16_t>(a, st);
+int launch_gate_norm_f(const GateNormArgs &a, bool aligned, hipStream_t st) {
+    if (a.fdt == DT_F32) return launch_gate_norm_typed<TX, float>(a, aligned, st);
+    return a.fdt == DT_F16 ? launch_gate_norm_typed<TX, half_t>(a, aligned, st) : launch_gate_norm_typed<TX, bf16_t>(a, aligned, st);
 }
 
 } // namespace
@@ -590,9 +644,10 @@ int gate_add_norm_check(GateNormArgs &a) {
 int launch_gate_add_norm(const GateNormArgs &a, hipStream_t st) {
     const uintptr_t at = (uintptr_t)a.x | (uintptr_t)a.f | (uintptr_t)a.x_out | (uintptr_t)a.y | (uintptr_t)a.mod | (uintptr_t)a.post_w |
                          (uintptr_t)a.post_b | (uintptr_t)a.pre_w | (uintptr_t)a.pre_b;
-    if (a.H % 8 == 0 && a.H <= 8192 && ((a.ldx | a.ldf | a.ldo | a.ldy) & 7) == 0 && (at & 31) == 0) {
-        if (a.xdt == DT_F32) return launch_gate_norm_f<float>(a, st);
-        return a.xdt == DT_F16 ? launch_gate_norm_f<half_t>(a, st) : launch_gate_norm_f<bf16_t>(a, st);
+    const bool aligned = a.H % 8 == 0 && ((a.ldx | a.ldf | a.ldo | a.ldy) & 7) == 0 && (at & 31) == 0;
+    if (a.H <= (aligned ? 8192u : 4096u)) {
+        if (a.xdt == DT_F32) return launch_gate_norm_f<float>(a, aligned, st);
+        return a.xdt == DT_F16 ? launch_gate_norm_f<half_t>(a, aligned, st) : launch_gate_norm_f<bf16_t>(a, aligned, st);
     }
     TSN_LAUNCH(gate_norm_any_kernel, dim3(std::min(a.rows, 1u << 20)), dim3(256), a.H * sizeof(float), st, a);
     TSN_HIP_CHECK(hipGetLastError());
