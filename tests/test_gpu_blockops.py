@@ -267,6 +267,12 @@ NORMS = [
     (3, 16, F32, F32, F32, 0, 0, 1, (2, 0, 1), False, None),
     (1003, 264, BF16, BF16, F32, 1, 1, 100, (2, 0, 1), True, None),
     (515, 72, F32, F16, F16, 2, 2, 5, (2, 0, 1), False, None),
+    (77, 333, F16, F32, BF16, 2, 2, 7, (2, 0, 1), True, None),             # one by one: one wave, four, eight
+    (19, 1777, BF16, F16, F32, 1, 2, 3, (2, 0, 1), True, (1777, 1779, 1781, 1783)),
+    (19, 2501, BF16, BF16, BF16, 2, 1, 1, (2, 0, 1), False, None),
+    (5, 4095, F32, F32, F32, 2, 2, 2, (2, 0, 1), True, None),
+    (5, 4097, F32, F16, F32, 1, 1, 2, (2, 0, 1), True, None),              # and past what registers hold
+    (5, 3328, F32, F16, F32, 1, 1, 2, (2, 0, 1), True, None),              # whole chunks, eight waves
 ]
 
 

@@ -202,8 +202,8 @@ __device__ __forceinline__ float group_sum(float v, float *red) {
     return v;
 }
 
-// Any width, stride and alignment (6352 rows of 1024: 38 us; whole chunks 15.7): a workgroup takes a row at a time, the row
-// (f, then x_out) in LDS as f32.
+// Rows that the kernel below does not hold in registers (over 8192 elements; over 4096 of any alignment): a workgroup takes
+// a row at a time, the row (f, then x_out) in LDS as f32 (6352 rows of 1024: 38 us; in registers 15.7).
 __global__ __launch_bounds__(256) void gate_norm_any_kernel(const GateNormArgs a) {
     extern __shared__ float row[];
     __shared__ float red[4];
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(256) void gate_norm_any_kernel(const GateNormArgs a
     }
 }
 
-// Rows of H % 8 == 0 aligned elements: W waves a row, NC chunks of eight elements a lane, the row in registers between
+// W waves a row, NC chunks of eight elements a lane, the row in registers between
 // one read and one write. A wave (a group of W) takes `per` rows one after the other and keeps what they share:
 // y = n(x_out) * A + B with A = pre_w (1 + scale), B = pre_b (1 + scale) + shift, and z's G = f_scale gate post_w, D =
 // f_scale gate post_b, made anew where a row of mod begins.
@@ -280,12 +280,13 @@ __global__ __launch_bounds__(256) void gate_norm_any_kernel(const GateNormArgs a
 // rows of 1024 with shared modulation, f32 and f16: 15.7 us, 5.0 TB/s; 8 rows: 3.5 us, a launch and a chain of four sums.
 // ANY: rows of any alignment and width: a lane's elements are 64 W apart, loaded and stored one by one, so that a wave's
 // access is of neighbours wherever a row begins (16-byte accesses at odd places: 20000 rows of 2501, bf16, each with its
-// row of mod XX -> 440 us; a row in LDS 379).
+// row of mod, 440 us; a row in LDS 380; so 185).
 template <typename TX, typename TF, int W, int NC, bool ONCE, bool ANY>
 __global__ __launch_bounds__(W > 1 ? 64 * W : 256, NC == 1 ? 4 : 2) void gate_norm_kernel(const GateNormArgs a, unsigned per) {
     constexpr int GROUPS = W > 1 ? 1 : 4;   // row groups of a workgroup
     __shared__ float red_all[GROUPS][W];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    // uniform where buffers are made (elsewhere it costs 1 to 2%)
+    const int wave = ANY ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : threadIdx.x >> 6, lane = threadIdx.x & 63;
     float *red = red_all[wave / W];
     const unsigned H = a.H, chunks = H / 8, first = (wave % W) * 64 + lane;
     // chunk c of the lane: elements 8 k on, k = 64 W c + first, or (ANY) 64 W (8 c + e) + first, e = 0..7
@@ -462,8 +463,9 @@ int launch_gate_norm_typed(const GateNormArgs &a, bool aligned, hipStream_t st) 
     }
     if (a.H <= 512) return launch_gate_norm_rows<TX, TF, 1, 1, false>(a, st);
     if (a.H <= 1024) return launch_gate_norm_rows<TX, TF, 2, 1, false>(a, st);
-    if (a.H <= 2048) return launch_gate_norm_rows<TX, TF, 2, 2, false>(a, st);
-    if (a.H <= 4096) return launch_gate_norm_rows<TX, TF, 4, 2, false>(a, st);
+    // two chunks a lane and half the waves: 20000 x 2504 with modulation a row 230 us, 178 as here; 6352 x 1536 23.2, 22.4
+    if (a.H <= 2048) return launch_gate_norm_rows<TX, TF, 4, 1, false>(a, st);
+    if (a.H <= 4096) return launch_gate_norm_rows<TX, TF, 8, 1, false>(a, st);
     return launch_gate_norm_rows<TX, TF, 8, 2, false>(a, st);   // to 8192
 }
 template <typename TX>
