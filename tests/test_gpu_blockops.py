@@ -271,7 +271,9 @@ NORMS = [
     (19, 1777, BF16, F16, F32, 1, 2, 3, (2, 0, 1), True, (1777, 1779, 1781, 1783)),
     (19, 2501, BF16, BF16, BF16, 2, 1, 1, (2, 0, 1), False, None),
     (5, 4095, F32, F32, F32, 2, 2, 2, (2, 0, 1), True, None),
-    (5, 4097, F32, F16, F32, 1, 1, 2, (2, 0, 1), True, None),              # and past what registers hold
+    (5, 4097, F32, F16, F32, 1, 1, 2, (2, 0, 1), True, None),              # sixteen
+    (7, 8191, BF16, F32, F16, 2, 2, 3, (2, 0, 1), True, None),
+    (5, 8193, F32, F16, F32, 1, 1, 2, (2, 0, 1), True, None),              # past what registers hold
     (5, 3328, F32, F16, F32, 1, 1, 2, (2, 0, 1), True, None),              # whole chunks, eight waves
 ]
 

@@ -202,8 +202,7 @@ __device__ __forceinline__ float group_sum(float v, float *red) {
     return v;
 }
 
-// Rows that the kernel below does not hold in registers (over 8192 elements; over 4096 of any alignment): a workgroup takes
-// a row at a time, the row (f, then x_out) in LDS as f32 (6352 rows of 1024: 38 us; in registers 15.7).
+// Rows that the kernel below does not hold in registers (over 8192 elements): a workgroup takes a row at a time, the row (f, then x_out) in LDS as f32 (6352 rows of 1024: 38 us; in registers 15.7).
 __global__ __launch_bounds__(256) void gate_norm_any_kernel(const GateNormArgs a) {
     extern __shared__ float row[];
     __shared__ float red[4];
@@ -455,11 +454,12 @@ int launch_gate_norm_rows(const GateNormArgs &a, hipStream_t st) {
 }
 template <typename TX, typename TF>
 int launch_gate_norm_typed(const GateNormArgs &a, bool aligned, hipStream_t st) {
-    if (!aligned) {   // to 4096; two chunks a lane would spill their addresses
+    if (!aligned) {
         if (a.H <= 512) return launch_gate_norm_rows<TX, TF, 1, 1, true>(a, st);
         if (a.H <= 1024) return launch_gate_norm_rows<TX, TF, 2, 1, true>(a, st);
         if (a.H <= 2048) return launch_gate_norm_rows<TX, TF, 4, 1, true>(a, st);
-        return launch_gate_norm_rows<TX, TF, 8, 1, true>(a, st);
+        if (a.H <= 4096) return launch_gate_norm_rows<TX, TF, 8, 1, true>(a, st);
+        return launch_gate_norm_rows<TX, TF, 16, 1, true>(a, st);   // to 8192
     }
     if (a.H <= 512) return launch_gate_norm_rows<TX, TF, 1, 1, false>(a, st);
     if (a.H <= 1024) return launch_gate_norm_rows<TX, TF, 2, 1, false>(a, st);
@@ -647,7 +647,7 @@ int launch_gate_add_norm(const GateNormArgs &a, hipStream_t st) {
     const uintptr_t at = (uintptr_t)a.x | (uintptr_t)a.f | (uintptr_t)a.x_out | (uintptr_t)a.y | (uintptr_t)a.mod | (uintptr_t)a.post_w |
                          (uintptr_t)a.post_b | (uintptr_t)a.pre_w | (uintptr_t)a.pre_b;
     const bool aligned = a.H % 8 == 0 && ((a.ldx | a.ldf | a.ldo | a.ldy) & 7) == 0 && (at & 31) == 0;
-    if (a.H <= (aligned ? 8192u : 4096u)) {
+    if (a.H <= 8192) {
         if (a.xdt == DT_F32) return launch_gate_norm_f<float>(a, aligned, st);
         return a.xdt == DT_F16 ? launch_gate_norm_f<half_t>(a, aligned, st) : launch_gate_norm_f<bf16_t>(a, aligned, st);
     }
