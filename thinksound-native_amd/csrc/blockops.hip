@@ -271,11 +271,10 @@ __global__ __launch_bounds__(256) void gate_norm_any_kernel(const GateNormArgs a
     }
 }
 
-// W waves a row, NC chunks of eight elements a lane, the row in registers between
-// one read and one write. A wave (a group of W) takes `per` rows one after the other and keeps what they share:
+// W waves a row, NC chunks of eight elements a lane, the row in registers between one read and one write. A wave (a group of W) takes `per` rows one after the other and keeps what they share:
 // y = n(x_out) * A + B with A = pre_w (1 + scale), B = pre_b (1 + scale) + shift, and z's G = f_scale gate post_w, D =
 // f_scale gate post_b, made anew where a row of mod begins.
-// Bound by memory: 32771 rows of 2048, bf16, each with its row of mod (1.34 GB): 227 us, 5.9 TB/s (a large copy: 6.2); 6352
+// Bound by memory: 32771 rows of 2048, bf16, each with its row of mod (1.34 GB): 229 us, 5.9 TB/s (a large copy: 6.2); 6352
 // rows of 1024 with shared modulation, f32 and f16: 15.7 us, 5.0 TB/s; 8 rows: 3.5 us, a launch and a chain of four sums.
 // ANY: rows of any alignment and width: a lane's elements are 64 W apart, loaded and stored one by one, so that a wave's
 // access is of neighbours wherever a row begins (16-byte accesses at odd places: 20000 rows of 2501, bf16, each with its
