@@ -183,7 +183,7 @@ int tsn_rope_axes(tsn_runtime *rt, const tsn_rope_axes_spec *spec, const void *x
  * from kv_len on may hold anything, infinities and NaN among it; those before are finite, and scaled scores below
  * 2^96.
  * f16 or bf16 in and out; scores, softmax statistics and sums in f32, probabilities rounded to the inputs' type for
- * the product with v. 16-byte aligned pointers and strides of a multiple of 8 elements run on MFMA, others a plain
+ * the product with v (f16: those below 2^-22 of a row's largest, 15.2 nats, to steps of at most 2^-32 of it). 16-byte aligned pointers and strides of a multiple of 8 elements run on MFMA, others a plain
  * kernel. out must not overlap an input. Where the rows alone do not fill the device, or their last round of workgroups
  * would be far from full, keys are shared out among workgroups: partial results go to the runtime's grow-on-demand
  * scratch and are joined in the order of the keys: same bits on every run. */

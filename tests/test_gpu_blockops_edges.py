@@ -1,0 +1,33 @@
+"""The block operators where rounding, range and the cuts of the work could lose something that evenly spread inputs do
+not show. References, tolerances and the call itself are those of test_gpu_blockops."""
+import numpy as np
+import pytest
+
+from test_gpu_blockops import BF16, F16, attn_case
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- one key far above the others
+
+@pytest.mark.parametrize("dt,hd", [(F16, 64), (F16, 32), (BF16, 64)])
+@pytest.mark.parametrize("nats", [10.0, 12.4, 14.2, 15.2])
+@pytest.mark.parametrize("at", ["first", "middle", "last"])
+@pytest.mark.parametrize("B,Sq,Sk,nh,heads", [
+    (2, 397, 397, 8, (0, 7)),          # few-row tiles of a workgroup each
+    (1, 1300, 3000, 50, (0, 49)),      # wide tiles
+    (1, 5, 20000, 2, None),            # keys shared out
+])
+def test_diff_attention_one_key_above(tsn, rt, dt, hd, nats, at, B, Sq, Sk, nh, heads):
+    """One key that every row prefers by 10 to 15 nats, with a value of zeros, and equal others that make up the
+    result: their probabilities of 2^-14.4 to 2^-22 of the largest are all rounded alike, so that a rounding step larger than the
+    type's own (f16 has steps of 2^-24 below 2^-14) shows as it is. The tolerance is the one of any other input."""
+    def make(r, q, k, v):
+        j = {"first": 0, "middle": Sk // 2 + 1, "last": Sk - 1}[at]
+        q[:], k[:] = 1.0, 0.0
+        k[:, j] = nats / np.sqrt(hd)
+        v[:] = 50.0 * (1.0 + np.abs(v))
+        v[:, j] = 0.0
+        return q, k, v
+
+    attn_case(tsn, rt, dt, B, Sq, Sk, nh, nh, hd, make=make, norm=False, heads=heads)
