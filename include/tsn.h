@@ -179,7 +179,7 @@ int tsn_rope_axes(tsn_runtime *rt, const tsn_rope_axes_spec *spec, const void *x
  * columns a head. hd is 32 or 64; lambda_init in [0, 1).
  * q_len, kv_len (device, [B], null: Sq, Sk; values are taken as 0 to Sq, 0 to Sk): row i < q_len of a sample sees
  * keys j < kv_len, with causal only j <= i + kv_len - q_len (its rows are the last of its keys, as new rows behind
- * a cache are). A row that sees no key gives zeros (so does any o of zeros, with an eps of 0 too). Rows of out from q_len on are left as they were. k and v rows
+ * a cache are). A row that sees no key gives zeros (so does any o of zeros, with an eps of 0 too; squares are summed in f32). Rows of out from q_len on are left as they were. k and v rows
  * from kv_len on may hold anything, infinities and NaN among it; those before are finite, and scaled scores below
  * 2^96.
  * f16 or bf16 in and out; scores, softmax statistics and sums in f32, probabilities rounded to the inputs' type for

@@ -31,3 +31,17 @@ def test_diff_attention_one_key_above(tsn, rt, dt, hd, nats, at, B, Sq, Sk, nh, 
         return q, k, v
 
     attn_case(tsn, rt, dt, B, Sq, Sk, nh, nh, hd, make=make, norm=False, heads=heads)
+
+
+# ---------------------------------------------------------------- values whose squares leave f32
+
+@pytest.mark.parametrize("hd", [64, 32])
+@pytest.mark.parametrize("Sq,Sk,nh,heads,pad", [
+    (40, 300, 4, None, 0), (1300, 1400, 50, (0, 49), 0), (1, 9000, 2, None, 0), (9, 300, 2, None, 1)])
+def test_diff_attention_small_values(tsn, rt, hd, Sq, Sk, nh, heads, pad):
+    """bf16 values of 2^-80 under the norm: their squares are zeros in f32, what is left of the mean square is eps
+    (2^-160 beside 1e-5), so that rows are scaled by 1/sqrt(eps) and not lost"""
+    def make(r, q, k, v):
+        return q, k, v * 2.0 ** -80
+
+    attn_case(tsn, rt, BF16, 1, Sq, Sk, nh, nh, hd, make=make, heads=heads, pad=(pad,) * 4)

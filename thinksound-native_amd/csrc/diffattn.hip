@@ -38,10 +38,12 @@ __device__ __forceinline__ float wave_lambda(const DiffAttnArgs &a, int h, int l
     return expf(d1) - expf(d2) + a.lambda_init;
 }
 
-// what the RMS norm multiplies a row of these squares with; a row without keys stays zero also where eps is
+// What the RMS norm multiplies a row of these squares with. Squares below f32's range (bf16 values under 2^-75) leave eps
+// alone; a row without keys stays zero also where eps is.
 template <int HD>
 __device__ __forceinline__ float rms_factor(const DiffAttnArgs &a, float squares) {
-    return squares == 0.0f ? 0.0f : (1.0f - a.lambda_init) / sqrtf(squares / (float)(2 * HD) + a.eps);
+    const float ms = squares / (float)(2 * HD) + a.eps;
+    return ms == 0.0f ? 0.0f : (1.0f - a.lambda_init) / sqrtf(ms);
 }
 
 // Any stride and alignment (two samples of 397 rows, 8 heads, f16: 133 us; whole chunks 11): one wave a row and head. A
