@@ -45,3 +45,16 @@ def test_diff_attention_small_values(tsn, rt, hd, Sq, Sk, nh, heads, pad):
         return q, k, v * 2.0 ** -80
 
     attn_case(tsn, rt, BF16, 1, Sq, Sk, nh, nh, hd, make=make, heads=heads, pad=(pad,) * 4)
+
+
+# ---------------------------------------------------------------- scores far from one
+
+@pytest.mark.parametrize("hd", [64, 32])
+@pytest.mark.parametrize("scale", [0.0, 2.0 ** -112])
+@pytest.mark.parametrize("Sq,Sk,nh,heads,pad", [
+    (40, 300, 4, None, 0), (1300, 1400, 50, (0, 49), 0), (1, 9000, 2, None, 0), (9, 300, 2, None, 1)])
+def test_diff_attention_large_products(tsn, rt, hd, scale, Sq, Sk, nh, heads, pad):
+    """bf16 q and k of 2^55: products of up to 2^120, which a scale of 0 turns into equal weights and one of 2^-112 into
+    scores of a few units"""
+    attn_case(tsn, rt, BF16, 1, Sq, Sk, nh, nh, hd, True, make=lambda r, q, k, v: (q * 2.0 ** 55, k * 2.0 ** 55, v),
+              heads=heads, pad=(pad,) * 4, scale=scale)

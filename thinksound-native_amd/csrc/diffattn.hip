@@ -385,7 +385,7 @@ __device__ __forceinline__ void load_rows(Rows<HD> &w, const DiffAttnArgs &a, in
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
-        for (int ks = 0; ks < L::KS; ++ks) w.q[j][ks] = *(const i32x4 *)(q + j * HD + ks * 16);
+        for (int ks = 0; ks < L::KS; ++ks) w.q[j][ks] = a.scale > 0.0f ? *(const i32x4 *)(q + j * HD + ks * 16) : i32x4{0, 0, 0, 0};
         w.m[j] = -1e30f;
         w.l[j] = 0.0f;
 #pragma unroll
@@ -587,7 +587,7 @@ struct Wide {
             const long long k0 = (long long)u * KB;
             load_tile<HD, NB>(lo, kp + k0 * ldk, vp + k0 * ldv, ldk, ldv, min(KB, nk - u * KB), lds + (u & 1) * STAGE + wave * NB * 1024, OP);
         };
-        const float c = a.scale > 0.0f ? a.scale * LOG2E : 1e-30f;   // a scale of 0 must not meet a masked score's infinity
+        const float c = a.scale > 0.0f ? a.scale * LOG2E : 1.0f;   // 0 must not meet a masked score's infinity: its queries are zeros instead
         const int end = min(t.u1, (keys + KB - 1) / KB);
         block_barrier();   // an earlier piece's LDS has been read
         if (t.u0 < end) issue(t.u0);
@@ -762,7 +762,7 @@ struct Few {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) qf[j][ks] = *(const i32x4 *)(q + j * HD + ks * 32);
+            for (int ks = 0; ks < KS; ++ks) qf[j][ks] = a.scale > 0.0f ? *(const i32x4 *)(q + j * HD + ks * 32) : i32x4{0, 0, 0, 0};
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[j][d] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
@@ -774,7 +774,7 @@ struct Few {
 #pragma unroll
             for (int i = 0; i < NQ; ++i) nw[i] = a.norm_w ? a.norm_w[col0 + 16 * (i >> 2) + (i & 3)] : 1.0f;
         }
-        const float c = a.scale > 0.0f ? a.scale * LOG2E : 1e-30f;   // a scale of 0 must not meet a masked score's infinity
+        const float c = a.scale > 0.0f ? a.scale * LOG2E : 1.0f;   // 0 must not meet a masked score's infinity: its queries are zeros instead
         // K row 8*(l16>>2) + (l16&3), chunk g4; V row 8*g4 + (l16>>2), column 4*(l16&3)
         const int kr = 8 * (l16 >> 2) + (l16 & 3), vr = 8 * g4 + (l16 >> 2);
         const unsigned kl = sk + kr * L::ROW + ((g4 ^ ksw(kr)) << 4);
