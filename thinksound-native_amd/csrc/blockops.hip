@@ -435,15 +435,9 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256, NC == 1 ? 4 : 2) void gate_no
 
 template <typename TX, typename TF, int W, int NC, bool ANY>
 int launch_gate_norm_rows(const GateNormArgs &a, hipStream_t st) {
-    constexpr unsigned GROUPS = W > 1 ? 1 : 4;
-    // Rows that share a row of mod in turn, so that the waves fill the device once (16 or 8 a CU): 6352 rows of 1024 take
-    // 22.2 us a row a wave, 16.6 us four rows a wave, 15.7 us four rows two waves (5.0 TB/s). A row of mod of its own:
-    // a row a group, and many groups waiting for a place.
-    constexpr unsigned AT_ONCE = NC == 1 ? 4096 : 2048;
-    const unsigned waves = (unsigned)(((unsigned long long)a.rows * W + AT_ONCE - 1) / AT_ONCE);
-    const unsigned per = std::max(a.mod_rows == 1 ? 1u : std::min(waves, 32u), (a.rows >> 22) + 1);   // a launch has less than 2^32 threads
-    const unsigned groups = a.rows / per + (a.rows % per != 0);
-    const dim3 grid((groups + GROUPS - 1) / GROUPS), block(W > 1 ? 64 * W : 256);
+    const GateNormCut cut = gate_norm_cut(a.rows, a.mod_rows, W, NC);
+    const dim3 grid(cut.grid), block(cut.block);
+    const unsigned per = cut.per;
     const bool once = passes_caches((size_t)a.rows * a.H * (2 * sizeof(TX) + sizeof(TF) + (a.y ? elem_bytes(a.ydt) : 0)));
     if constexpr (ANY) TSN_LAUNCH((gate_norm_kernel<TX, TF, W, NC, false, true>), grid, block, 0, st, a, per);
     else if (once) TSN_LAUNCH((gate_norm_kernel<TX, TF, W, NC, true, false>), grid, block, 0, st, a, per);
@@ -593,6 +587,22 @@ int launch_rope_axes(const RopeAxesArgs &c, hipStream_t st) {
     TSN_LAUNCH(rope_axes_any_kernel, dim3((unsigned)std::min<unsigned long long>((n + 255) / 256, 1 << 20)), dim3(256), 0, st, a);
     TSN_HIP_CHECK(hipGetLastError());
     return TSN_OK;
+}
+
+// Rows that share a row of mod in turn, so that the waves fill the device once (16 or 8 a CU): 6352 rows of 1024 take
+// 22.2 us a row a wave, 16.6 us four rows a wave, 15.7 us four rows two waves (5.0 TB/s). A row of mod of its own:
+// a row a group, and many groups waiting for a place. A launch has less than 2^32 threads.
+GateNormCut gate_norm_cut(uint32_t rows, uint32_t mod_rows, unsigned waves, unsigned chunks) {
+    const unsigned long long at_once = chunks == 1 ? 4096 : 2048;
+    const unsigned groups_of = waves > 1 ? 1 : 4;   // row groups of a workgroup
+    GateNormCut c;
+    c.block = waves > 1 ? 64 * waves : 256;
+    const unsigned most = 0xFFFFFFFFu / c.block * groups_of;   // groups of a launch
+    const unsigned long long turns = ((unsigned long long)rows * waves + at_once - 1) / at_once;
+    c.per = std::max(mod_rows == 1 ? 1u : (unsigned)std::min(turns, 32ULL), rows / most + (rows % most != 0));
+    const unsigned groups = rows / c.per + (rows % c.per != 0);
+    c.grid = (groups + groups_of - 1) / groups_of;
+    return c;
 }
 
 int gate_add_norm_check(GateNormArgs &a) {

@@ -512,5 +512,11 @@ int launch_rope_axes(const RopeAxesArgs &a, hipStream_t st);
 size_t diff_attention_bytes(const DiffAttnArgs &a);
 int launch_diff_attention(const DiffAttnArgs &a, void *ws, size_t ws_bytes, hipStream_t st);
 int launch_gate_add_norm(const GateNormArgs &a, hipStream_t st);
+// how rows of up to 8192 are launched: `waves` waves a row, `chunks` chunks of eight elements a lane; a group of waves takes
+// `per` rows in turn, four groups a workgroup where a group is one wave
+struct GateNormCut {
+    unsigned per, grid, block;
+};
+GateNormCut gate_norm_cut(uint32_t rows, uint32_t mod_rows, unsigned waves, unsigned chunks);
 
 } // namespace tsn
