@@ -165,3 +165,47 @@ def test_wrappers_check_array_sizes(tsn):
         tsn.rope_axes_spec(tsn.F32, 1, 1, 64, (8,) * 5, (1e4,) * 5)
     with pytest.raises(ValueError):
         tsn.rope_axes_spec(tsn.F32, 1, 1, 64, (8, 8), (1e4,))
+
+
+@pytest.mark.parametrize("kw,word", [
+    # one sample: its stride is not taken
+    (dict(B=1, bsq=5, out=BASE + 2048, ldo=2048, ldq=2048), NULL_RT),
+    (dict(B=1, bso=77, out=BASE + 2048, ldo=2048, ldq=2048), NULL_RT),
+    (dict(B=1, bsq=5, out=BASE + 2046, ldo=2048, ldq=2048), "overlaps an input"),
+    # one row: its stride is not taken (q and out of every sample in one row of 2048)
+    (dict(Sq=1, ldq=1032, ldo=1024, bsq=2048, bso=2048, out=BASE + 2048), NULL_RT),
+    (dict(Sq=1, ldq=1032, ldo=1024, bsq=2048, bso=2048, out=BASE + 2000), "overlaps an input"),
+    # samples between each other's rows: [row][sample][q | out]
+    (dict(ldq=4096, ldo=4096, bsq=2048, bso=2048, out=BASE + 2048), NULL_RT),
+    (dict(ldq=4096, ldo=4096, bsq=2048, bso=2048, out=BASE + 2040), "overlaps an input"),
+    (dict(ldq=4096, ldo=4096, bsq=2048, bso=2048, out=BASE + 2056), "overlaps an input"),
+    (dict(ldq=4096, ldo=4096, bsq=2048, bso=2040, out=BASE + 2048), "overlaps an input"),
+    (dict(ldq=2048, ldo=4096, out=BASE + 2048), NULL_RT),             # every other row of q's
+    (dict(ldq=2048, ldo=4096, bso=40 * 4096 + 1024, out=BASE + 2048), "overlaps an input"),
+])
+def test_diff_attention_shared_rows(tsn, kw, word):
+    """out in the same buffer as q is taken wherever no element is shared, whatever strides are not used"""
+    rc, msg = attn(tsn, **kw)
+    assert rc == 1 and word in msg, (rc, msg)
+
+
+def test_windows_brute_force(tsn):
+    """q and out a few rows and samples in one small buffer, against the elements themselves: no call is taken in which two
+    of out's elements, or one of out's and one of q's, are the same"""
+    r = np.random.default_rng(3)
+    taken = 0
+    for _ in range(4000):
+        B, Sq, nh = int(r.integers(1, 4)), int(r.integers(1, 4)), 1
+        w = 64   # 2 * nh * hd of width 32
+        ldq, ldo = (int(w * r.integers(1, 5) + r.choice([0, 0, 0, 8])) for _ in range(2))
+        bsq, bso = (int(w * r.integers(1, 12)) for _ in range(2))
+        at = int(w * r.integers(0, 6) + r.choice([0, 0, 0, 4, 60]))
+        q = {b * bsq + i * ldq + c for b in range(B) for i in range(Sq) for c in range(w)}
+        o = [at + b * bso + i * ldo + c for b in range(B) for i in range(Sq) for c in range(w)]
+        rc, msg = attn(tsn, B=B, Sq=Sq, nh=nh, nkv=1, hd=32, ldq=ldq, ldo=ldo, bsq=bsq, bso=bso, out=BASE + 2 * at)
+        if NULL_RT in msg:
+            taken += 1
+            assert len(set(o)) == len(o) and not q & set(o), (B, Sq, ldq, ldo, bsq, bso, at)
+        else:
+            assert "overlap" in msg, msg
+    assert taken > 400

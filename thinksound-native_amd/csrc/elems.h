@@ -1,6 +1,8 @@
 // elems.h — element types of the block operators: f32, f16 and bf16 rows as floats, and host checks
 // that two strided row windows share no element.
 #pragma once
+#include <numeric>
+
 #include "tsn_common.h"
 
 namespace tsn {
@@ -48,14 +50,20 @@ inline Window window(const void *p, size_t elem, unsigned long long width, unsig
                      unsigned long long rows, unsigned long long bs = 0, unsigned long long samples = 1) {
     return Window{p, width * elem, ld * elem, rows, bs * elem, samples};
 }
-// Whether two windows may share bytes. Apart from each other, or columns of the same rows (equal row strides, sample
-// strides whole rows, and column ranges that do not meet): they do not.
+// Whether two windows may share bytes. They do not if they are apart from each other, or if all rows of both begin at one
+// place each within g bytes, g dividing every stride that is taken, and these column ranges do not meet (columns of the same
+// rows; samples between each other's rows).
 inline bool windows_meet(const Window &a, const Window &b) {
     const unsigned long long pa = (unsigned long long)a.p, pb = (unsigned long long)b.p;
     if (pa >= b.end() || pb >= a.end()) return false;
-    if (a.ld != b.ld || a.bs % a.ld || b.bs % a.ld) return true;
-    const unsigned long long d = (pb >= pa ? pb - pa : a.ld - (pa - pb) % a.ld) % a.ld;   // b's first column after a's
-    return !(d >= a.width && d + b.width <= a.ld);
+    unsigned long long g = 0;
+    for (const Window *w : {&a, &b}) {
+        if (w->rows > 1) g = std::gcd(g, w->ld);
+        if (w->samples > 1) g = std::gcd(g, w->bs);
+    }
+    if (g == 0) return true;   // a row each
+    const unsigned long long d = (pb >= pa ? pb - pa : g - (pa - pb) % g) % g;   // b's first column after a's
+    return !(d >= a.width && d + b.width <= g);
 }
 
 } // namespace tsn
