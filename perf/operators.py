@@ -4,6 +4,10 @@ norms on both sides of the block, as a program calls them: the cases, their inpu
 Device memory is torch's: the library takes device pointers, so a torch tensor's storage serves as input
 or output of any call. The plain form computes in 32 bits (rotary angles in 64) from elementary torch
 operations and rounds once; `own` makes the calls of the package instead.
+
+The package's calls run on a stream of its runtime, which neither waits for torch's streams nor is waited for by them:
+`prepare` waits for the device before and after it makes tensors, and a program that lets torch read a result, or drops a
+state, waits for the device first (torch.cuda.synchronize). Passes over the same state follow each other.
 """
 import ctypes
 import math
@@ -210,7 +214,10 @@ def _plan(case):
 
 
 def prepare(case, seed):
-    return State(case, seed)
+    torch.cuda.synchronize()   # a call on an earlier state may still be using memory that torch hands out again
+    st = State(case, seed)
+    torch.cuda.synchronize()   # inputs and cleared outputs are there before a call on another stream
+    return st
 
 
 def run(st):
