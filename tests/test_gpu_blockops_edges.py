@@ -58,3 +58,23 @@ def test_diff_attention_large_products(tsn, rt, hd, scale, Sq, Sk, nh, heads, pa
     scores of a few units"""
     attn_case(tsn, rt, BF16, 1, Sq, Sk, nh, nh, hd, True, make=lambda r, q, k, v: (q * 2.0 ** 55, k * 2.0 ** 55, v),
               heads=heads, pad=(pad,) * 4, scale=scale)
+
+
+# ---------------------------------------------------------------- rows that are not whole 16-byte chunks
+
+@pytest.mark.parametrize("hd", [64, 32])
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("B,Sq,Sk,nh,nkv,causal,ql,kl,shared_lambda", [
+    (2, 34, 200, 4, 2, False, None, None, True),
+    (3, 40, 130, 4, 4, False, [40, 0, 7], [130, 64, 0], False),
+    (3, 70, 70, 6, 2, True, [70, 33, 1], [70, 33, 1], False),
+    (2, 1, 1000, 4, 1, True, None, [1000, 999], False),
+    (2, 33, 65, 2, 2, True, [33, 20], [20, 65], True),       # rows before the first key
+    (1, 1, 1, 1, 1, False, None, None, True),
+])
+def test_diff_attention_odd_places(tsn, rt, dt, hd, norm, B, Sq, Sk, nh, nkv, causal, ql, kl, shared_lambda):
+    """odd strides and columns: the kernel that reads element by element, in each of its widths and types, under every mask,
+    with and without its norm"""
+    attn_case(tsn, rt, dt, B, Sq, Sk, nh, nkv, hd, causal, ql, kl, lam_heads=1 if shared_lambda else nh, norm=norm,
+              junk=np.nan, pad=(1, 3, 5, 7), col=1)
