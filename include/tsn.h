@@ -181,7 +181,7 @@ int tsn_rope_axes(tsn_runtime *rt, const tsn_rope_axes_spec *spec, const void *x
  * keys j < kv_len, with causal only j <= i + kv_len - q_len (its rows are the last of its keys, as new rows behind
  * a cache are). A row that sees no key gives zeros (so does any o of zeros, with an eps of 0 too; squares are summed in f32). Rows of out from q_len on are left as they were. k and v rows
  * from kv_len on may hold anything, infinities and NaN among it; those before are finite,
- * their products with q finite in f32, and scaled scores below 2^96.
+ * their products with q finite in f32, scaled scores below 2^96 and values below 2^60.
  * f16 or bf16 in and out; scores, softmax statistics and sums in f32, probabilities rounded to the inputs' type for
  * the product with v (f16: those below 2^-22 of a row's largest, 15.2 nats, to steps of at most 2^-32 of it). 16-byte aligned pointers and strides of a multiple of 8 elements run on MFMA, others a plain
  * kernel. out must not overlap an input. Where the rows alone do not fill the device, or their last round of workgroups

@@ -78,3 +78,15 @@ def test_diff_attention_odd_places(tsn, rt, dt, hd, norm, B, Sq, Sk, nh, nkv, ca
     with and without its norm"""
     attn_case(tsn, rt, dt, B, Sq, Sk, nh, nkv, hd, causal, ql, kl, lam_heads=1 if shared_lambda else nh, norm=norm,
               junk=np.nan, pad=(1, 3, 5, 7), col=1)
+
+
+# ---------------------------------------------------------------- values far above one
+
+@pytest.mark.parametrize("hd", [64, 32])
+@pytest.mark.parametrize("Sq,Sk,nh,heads,pad", [
+    (40, 300, 4, None, 0), (1300, 1400, 50, (0, 49), 0), (1, 9000, 2, None, 0), (9, 300, 2, None, 1)])
+def test_diff_attention_large_values(tsn, rt, hd, Sq, Sk, nh, heads, pad):
+    """bf16 values of up to 2^57 under the norm (their squares add up to less than 2^128), of up to 2^113 without it"""
+    for power, norm in ((55, True), (111, False)):
+        attn_case(tsn, rt, BF16, 1, Sq, Sk, nh, nh, hd, heads=heads, make=lambda r, q, k, v: (q, k, np.clip(v, -4, 4) * 2.0 ** power),
+                  pad=(pad,) * 4, norm=norm)

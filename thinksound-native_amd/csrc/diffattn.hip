@@ -321,23 +321,25 @@ __device__ __forceinline__ float exp_scores(const floatx16 &s, float c, float m,
     return sum;
 }
 // Probabilities of 32 keys, to the reference m of earlier ones. A reference may lie below a score as long as no
-// probability nears f16's range: a lane's 16 add up to no more than MOST. Only where one exceeds that (the first block:
+// probability nears f16's range: a lane's 16 add up to no more than `most`. Only where one exceeds that (the first block:
 // m = -1e30) are the maxima taken, the references moved and O and the sums scaled; most blocks take no maximum at all.
-// A reference is set BELOW (log2 units) below the maximum, so that f16 probabilities are subnormal, in steps of 2^-24 of 1,
+// For f16 a reference is set 2^8 (`below`) under the maximum, so that probabilities are subnormal, in steps of 2^-24 of 1,
 // from 2^-22 of the largest down (15.2 nats) and not from 2^-14: with one key 14.2 nats above 700 others of equal scores
-// the others' joint weight was off by 3.7% of itself. Against references at the maximum and MOST 2^12 8 takes 0 to 1%
-// longer (957, 946 us for 12289 rows, 150.5, 149.1 for 16 x 1101), 10 takes 1 to 4% (references move more often).
-constexpr float BELOW = 8.0f, MOST = 32768.0f;
+// the others' joint weight was off by 3.7% of itself. Time (12289 rows; 16 x 1101): with references at the maximum and sums to
+// 2^12 957 and 150.5 us, 2^8 under it 946 and 149.1, 2^10 under it 959 and 154.4 (they move more often). bf16 has f32's range.
+template <typename T> struct Reference;
+template <> struct Reference<half_t> { static constexpr float below = 8.0f, most = 32768.0f; };
+template <> struct Reference<bf16_t> { static constexpr float below = 0.0f, most = 4096.0f; };
 template <typename T, int HD>
 __device__ __forceinline__ void probs(Rows<HD> &w, const floatx16 (&s)[2], i32x4 (&p)[2][2], float c) {
     float sum[2] = {exp_scores<T>(s[0], c, w.m[0], p[0]), exp_scores<T>(s[1], c, w.m[1], p[1])};
-    if (__builtin_amdgcn_ballot_w64(!(fmaxf(sum[0], sum[1]) <= MOST)) != 0) {
+    if (__builtin_amdgcn_ballot_w64(!(fmaxf(sum[0], sum[1]) <= Reference<T>::most)) != 0) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             float t = fmaxf(fmaxf(s[j][0], s[j][1]), s[j][2]);
 #pragma unroll
             for (int r = 3; r < 15; r += 2) t = fmaxf(fmaxf(t, s[j][r]), s[j][r + 1]);
-            const float mn = fmaxf(w.m[j], pair_max(fmaxf(t, s[j][15])) * c - BELOW);
+            const float mn = fmaxf(w.m[j], pair_max(fmaxf(t, s[j][15])) * c - Reference<T>::below);
             const float al = __builtin_amdgcn_exp2f(w.m[j] - mn);
             w.m[j] = mn;
             w.l[j] *= al;
@@ -815,12 +817,12 @@ struct Few {
             }
             i32x4 p[2];
             float sum[2] = {exps(s[0], c, m[0], p[0]), exps(s[1], c, m[1], p[1])};
-            if (__builtin_amdgcn_ballot_w64(!(fmaxf(sum[0], sum[1]) <= MOST)) != 0) {   // as in probs
+            if (__builtin_amdgcn_ballot_w64(!(fmaxf(sum[0], sum[1]) <= Reference<T>::most)) != 0) {   // as in probs
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const float top = fmaxf(fmaxf(fmaxf(s[j][0][0], s[j][0][1]), fmaxf(s[j][0][2], s[j][0][3])),
                                             fmaxf(fmaxf(s[j][1][0], s[j][1][1]), fmaxf(s[j][1][2], s[j][1][3])));
-                    const float mn = fmaxf(m[j], quad_max(top) * c - BELOW);
+                    const float mn = fmaxf(m[j], quad_max(top) * c - Reference<T>::below);
                     const float al = __builtin_amdgcn_exp2f(m[j] - mn);
                     m[j] = mn;
                     l[j] *= al;
