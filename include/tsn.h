@@ -148,8 +148,8 @@ int tsn_attention(tsn_runtime *rt, const float *qkv, float *out, uint32_t S, uin
 
 /* ---------------- transformer block operators beside the launchers above (no reference counterpart) ----------------
  * Inference forms, all on the runtime's stream. Each reads its spec (host memory) before it returns. Argument errors
- * are found before anything is launched; rows are less than 2^31. Only tsn_diff_attention uses device memory of its own: the runtime's
- * grow-on-demand scratch (see there). */
+ * are found before anything is launched; rows are less than 2^31. Only tsn_diff_attention uses device memory of its own:
+ * the runtime's grow-on-demand scratch (see there). */
 
 /* Rotary positions with several axes (time, height, width): tsn_rope_pairs for clip rows cut from frames. Pair i of
  * axis a of every head of row r turns by
@@ -179,14 +179,16 @@ int tsn_rope_axes(tsn_runtime *rt, const tsn_rope_axes_spec *spec, const void *x
  * columns a head. hd is 32 or 64; lambda_init in [0, 1).
  * q_len, kv_len (device, [B], null: Sq, Sk; values are taken as 0 to Sq, 0 to Sk): row i < q_len of a sample sees
  * keys j < kv_len, with causal only j <= i + kv_len - q_len (its rows are the last of its keys, as new rows behind
- * a cache are). A row that sees no key gives zeros (so does any o of zeros, with an eps of 0 too; squares are summed in f32). Rows of out from q_len on are left as they were. k and v rows
- * from kv_len on may hold anything, infinities and NaN among it; those before are finite,
- * their products with q finite in f32, scaled scores below 2^96 and values below 2^60.
+ * a cache are). A row that sees no key gives zeros (so does any o of zeros, with an eps of 0 too; squares are summed in
+ * f32). Rows of out from q_len on are left as they were. k and v rows from kv_len on may hold anything, infinities and
+ * NaN among it; those before are finite, their products with q finite in f32, scaled scores below 2^96 and values below
+ * 2^60. A scale of 0 gives equal weights.
  * f16 or bf16 in and out; scores, softmax statistics and sums in f32, probabilities rounded to the inputs' type for
- * the product with v (f16: those below 2^-22 of a row's largest, 15.2 nats, to steps of at most 2^-32 of it). 16-byte aligned pointers and strides of a multiple of 8 elements run on MFMA, others a plain
- * kernel. out must not overlap an input. Where the rows alone do not fill the device, or their last round of workgroups
- * would be far from full, keys are shared out among workgroups: partial results go to the runtime's grow-on-demand
- * scratch and are joined in the order of the keys: same bits on every run. */
+ * the product with v (f16: those below 2^-22 of a row's largest, 15.2 nats, to steps of at most 2^-32 of it). 16-byte
+ * aligned pointers and strides of a multiple of 8 elements run on MFMA, others a plain kernel. out must not overlap an
+ * input (columns of the same rows do not). Where the rows alone do not fill the device, or their last round of
+ * workgroups would be far from full, keys are shared out among workgroups: partial results go to the runtime's
+ * grow-on-demand scratch and are joined in the order of the keys: same bits on every run. */
 typedef struct {
     int dtype;                    /* q, k, v and out: TSN_F16 or TSN_BF16 */
     uint32_t B, Sq, Sk;           /* samples, rows and keys of each */

@@ -81,8 +81,9 @@ __global__ __launch_bounds__(256) void rope_axes_any_kernel(const RopeKernelArgs
     }
 }
 
-// Whole chunks of VE elements (16 bytes; 8 or two elements where halves of axes do not divide into more): a workgroup takes rb rows, computes the cosines and sines of their pairs once (in LDS, for all
-// heads) while its first chunks are under way, and turns them. An item is a chunk (neighbouring pairs) or the two
+// Whole chunks of VE elements (16 bytes; 8 or two elements where halves of axes do not divide into more): a workgroup takes
+// rb rows, computes the cosines and sines of their pairs once (in LDS, for all heads) while its first chunks are under way,
+// and turns them. An item is a chunk (neighbouring pairs) or the two
 // chunks that hold a pair's halves; behind the axes a chunk is copied. per_head items a head, per_row a row;
 // the magic numbers divide by them.
 // Bound by memory: 32768 rows of 32 heads of 64, f16, 269 MB: 44.3 us, 6.05 TB/s (a large copy: 6.2); 4999 rows of 24
@@ -202,7 +203,8 @@ __device__ __forceinline__ float group_sum(float v, float *red) {
     return v;
 }
 
-// Rows that the kernel below does not hold in registers (over 8192 elements): a workgroup takes a row at a time, the row (f, then x_out) in LDS as f32 (6352 rows of 1024: 38 us; in registers 15.7).
+// Rows that the kernel below does not hold in registers (over 8192 elements): a workgroup takes a row at a time, the row (f,
+// then x_out) in LDS as f32 (6352 rows of 1024: 38 us; in registers 15.7).
 __global__ __launch_bounds__(256) void gate_norm_any_kernel(const GateNormArgs a) {
     extern __shared__ float row[];
     __shared__ float red[4];
@@ -271,7 +273,8 @@ __global__ __launch_bounds__(256) void gate_norm_any_kernel(const GateNormArgs a
     }
 }
 
-// W waves a row, NC chunks of eight elements a lane, the row in registers between one read and one write. A wave (a group of W) takes `per` rows one after the other and keeps what they share:
+// W waves a row, NC chunks of eight elements a lane, the row in registers between one read and one write. A wave (a group of
+// W) takes `per` rows one after the other and keeps what they share:
 // y = n(x_out) * A + B with A = pre_w (1 + scale), B = pre_b (1 + scale) + shift, and z's G = f_scale gate post_w, D =
 // f_scale gate post_b, made anew where a row of mod begins.
 // Bound by memory: 32771 rows of 2048, bf16, each with its row of mod (1.34 GB): 229 us, 5.9 TB/s (a large copy: 6.2); 6352
@@ -459,7 +462,9 @@ int launch_gate_norm_typed(const GateNormArgs &a, bool aligned, hipStream_t st) 
     // two chunks a lane and half the waves: 20000 x 2504 with modulation a row 230 us, 178 as here; 6352 x 1536 23.2, 22.4
     if (a.H <= 2048) return launch_gate_norm_rows<TX, TF, 4, 1, false>(a, st);
     if (a.H <= 4096) return launch_gate_norm_rows<TX, TF, 8, 1, false>(a, st);
-    return launch_gate_norm_rows<TX, TF, 8, 2, false>(a, st);   // to 8192
+    // to 8192. Sixteen waves of one chunk, bf16, beside this (us): 6352 x 5120 with shared modulation 58.8, 56.7, with a row's
+    // own 136, 157 (floors 42, 104); 6352 x 8192 88, 88 and 193, 200 (67, 167); f32 and f16 87.8, 89.3 and 160, 171 at 5120.
+    return launch_gate_norm_rows<TX, TF, 8, 2, false>(a, st);
 }
 template <typename TX>
 int launch_gate_norm_f(const GateNormArgs &a, bool aligned, hipStream_t st) {

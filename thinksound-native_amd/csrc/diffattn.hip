@@ -5,7 +5,8 @@
 // softmax), and the two are joined once both sums are known.
 //
 // Work of a pair (row, key) that a head sees: 4 hd operations for both maps' scores, 8 hd for their products with V (joined
-// before it the maps need 4 hd, but both sums first, so the scores twice: 12 hd as well), two exponentials. Long contexts are bound by these under the card's power limit, one new row by reading its cache.
+// before it the maps need 4 hd, but both sums first, so the scores twice: 12 hd as well), two exponentials. Long contexts
+// are bound by these under the card's power limit, one new row by reading its cache.
 #include <math.h>
 
 #include <algorithm>
@@ -557,10 +558,12 @@ __device__ __forceinline__ bool ranked_part(const DiffAttnArgs &a, const DiffPla
 
 // A workgroup's worker: 128 rows, 32 a wave. The four waves share K and V tiles of 64 keys, two stages in LDS: the next is
 // loaded while one is worked on. Two workgroups a CU (hd 32: three), one's matrix products cover the other's softmax.
-// Measured: 12289 rows and keys, 8 heads, hd 64, f16: 938 us, 990 TFLOP/s of the 12 hd operations a pair (matrix units half
-// busy at 1.9 GHz, which the power limit leaves; a library bf16 product of 8192^3 reaches 1259). 1101 rows, 128 heads: 150
-// us, 790. One wave a SIMD, the products of a step beside the softmax of the one before: 1500 us for the first; 64 rows a
-// workgroup and two waves that share the keys: spills. Causal, hd 32, 677 to 2047 rows of four heads a key: 48.6 us.
+// Measured (calls in a row; the first hundred after a pause take up to 18% longer, until the clocks have settled): 12289
+// rows and keys, 8 heads, hd 64, f16: 950 to 967 us, 960 to 980 TFLOP/s of the 12 hd operations a pair (matrix units half
+// busy at 1.9 GHz, which the power limit leaves; a library bf16 product of 8192^3 reaches 1259). 1101 rows, 128 heads, bf16: 149
+// to 152 us, 790 (matrix units 0.31 busy: half a round of tiles at the end, 18 key tiles between a tile's start and end). One
+// wave a SIMD, the products of a step beside the softmax of the one before: 1500 us for the first; 64 rows a workgroup and
+// two waves that share the keys: spills. Causal, hd 32, 677 to 2047 rows of four heads a key, f16: 50.3 us.
 template <typename T, int HD>
 struct Wide {
     using L = Lay<HD>;
@@ -686,7 +689,7 @@ __device__ __forceinline__ float quad_sum(float v) {
     return pair_sum(__uint_as_float(p[0]) + __uint_as_float(p[1]));
 }
 // Measured: 64 caches of 2048 to 8192 keys, 4 heads of 4 rows, bf16: 121 us with the join, 5.8 TB/s of K and V (a large copy
-// on this card: 6.2); one row over 4099 keys, 8 heads: 12.2 us, 7.2 of it this kernel, all latency; two samples of 397
+// on this card: 6.2); one row over 4099 keys, 8 heads: 12.3 us (traced: 8.6 and 4.2 for the join), all latency; two samples of 397
 // rows, 8 heads: 11 us (32 rows a workgroup that share their tiles: 13.1).
 template <typename T, int HD>
 struct Few {
@@ -746,7 +749,9 @@ struct Few {
         auto load = [&](int u, const char *p, unsigned ld, const unsigned (&o)[NB], unsigned to) {
             const int k0 = u * KB + 32 * kw, n = min(32, nk - k0) - 1;   // rows behind the last key read as zero
             const i32x4 rs = buffer(p + (long long)k0 * ld, n < 0 ? 0u : (unsigned)n * ld + L::ROW);
-            // a head with one tile reads its keys once (64 caches of 8192 keys: 140 -> 126 us past the caches)
+            // A head with one tile reads its keys once: past the caches, at every size. Bytes of K and V, us past them and
+            // through them: 16.8 MB 12.9, 13.5; 67 MB 30.0, 31.4; 268 MB 46.6, 53.3; 1074 MB 168, 185, with other
+            // caches read in between, as between the steps of a model. Read again at once: 10.9, 10.9; 28.9, 21.9; 46.0, 44.2.
             if (pl.ntile == 1) {
 #pragma unroll
                 for (int i = 0; i < NB; ++i) dma16(rs, o[i], 0, to + i * 1024, true);
