@@ -330,8 +330,8 @@ __device__ __forceinline__ float exp_scores(const floatx16 &s, float c, float m,
 // m = -1e30) are the maxima taken, the references moved and O and the sums scaled; most blocks take no maximum at all.
 // For f16 a reference is set 2^8 (`below`) under the maximum, so that probabilities are subnormal, in steps of 2^-24 of 1,
 // from 2^-22 of the largest down (15.2 nats) and not from 2^-14: with one key 14.2 nats above 700 others of equal scores
-// the others' joint weight was off by 3.7% of itself. Time (12289 rows; 16 x 1101): with references at the maximum and sums to
-// 2^12 957 and 150.5 us, 2^8 under it 946 and 149.1, 2^10 under it 959 and 154.4 (they move more often). bf16 has f32's range.
+// the others' joint weight was off by 3.7% of itself. It takes 1% (12289 rows: references at the maximum and sums to 2^12 946
+// us, 2^8 under it 957, 2^10 under it 959 to 964: the further down, the more often they move). bf16 has f32's range.
 template <typename T> struct Reference;
 template <> struct Reference<half_t> { static constexpr float below = 8.0f, most = 32768.0f; };
 template <> struct Reference<bf16_t> { static constexpr float below = 0.0f, most = 4096.0f; };
